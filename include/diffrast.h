@@ -498,6 +498,89 @@ DR_API dr_status dr_adam_step(dr_ctx* ctx, float* param, const float* grad,
                        float lr, float beta1, float beta2, float eps,
                        float bias_c1, float bias_c2);
 
+/* ---- gradient norm, clipping and AdamW over many tensors ---------------- */
+
+/* Element types of the tensors below. */
+typedef enum dr_dtype { DR_F32 = 0, DR_BF16 = 1, DR_F16 = 2 } dr_dtype;
+
+/* A flat tensor of n elements (data may be NULL when n == 0). */
+typedef struct dr_grad_tensor {
+  void* data;
+  int64_t n;
+  int32_t type; /* dr_dtype */
+  int32_t reserved; /* 0 */
+} dr_grad_tensor;
+
+/* Device scratch of the three entry points below, in bytes: the partial sums
+ * of a norm over `count` tensors on this context's device.  The caller owns it
+ * and needs not clear it; calls that may overlap on the GPU (two streams, two
+ * captured graphs) each need their own. */
+DR_API size_t dr_grad_norm_work_bytes(const dr_ctx* ctx, int count);
+
+/* *norm (device) = the 2-norm over all elements of `count` tensors, of any mix
+ * of types.  Squares are formed and summed in 64 bits in a fixed order, so the
+ * result neither overflows before the norm itself does nor changes from run to
+ * run.  `grads` is a host array; it is read before the call returns. */
+DR_API dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, float* norm,
+                       void* work);
+
+/* dr_grad_norm, then every element times min(1, max_norm / (norm + 1e-6)) in
+ * place (nothing is written when that factor is 1).  A NaN or infinite norm
+ * gives the factors NaN and 0 that the formula does. */
+DR_API dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count,
+                            double max_norm, float* norm, void* work);
+
+/* One tensor of an AdamW step.  With state_bits = 32, m and v are float [n].
+ * With state_bits = 8, m and v hold e4m3 codes [n] of the first moment and of
+ * the SQUARE ROOT of the second, and m_scale / v_scale the float factor of each
+ * block of 256 elements [ceil(n / 256)]: value = code * scale, scale = (largest
+ * magnitude in the block) / 448, 0 for a largest magnitude below 2^-100 and NaN
+ * for one that is not finite.  All state is 0 before the first step. */
+typedef struct dr_adamw_tensor {
+  void* param;        /* [n] of param_type, updated in place */
+  const void* grad;   /* [n] of grad_type */
+  float* master;      /* NULL, or the fp32 weights [n] that `param` is rounded from */
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  double* clock;      /* device [4]: t, beta1^t, beta2^t, unused; 0, 1, 1, 0 before the first step */
+  int64_t n;
+  double lr_ratio;    /* this tensor's learning rate / the step's */
+  double weight_decay;
+  uint32_t seed;      /* of the stochastic rounding (state_bits = 8); differs between tensors */
+  int32_t param_type; /* dr_dtype */
+  int32_t grad_type;  /* dr_dtype: param_type, DR_F32, or any when param_type is DR_F32 */
+  int32_t reserved;   /* 0 */
+} dr_adamw_tensor;
+
+/* One AdamW step of `count` tensors in place.  For step t = clock[0] + 1 of
+ * each tensor, each operation rounded to float (the factors in t in double):
+ *   g = coef * grad
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr wd) - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * and clock advances to t.  lr = lr_ratio * (*lr_device, a device float read by
+ * the step, or `lr` when lr_device is NULL).
+ * max_norm > 0: coef = min(1, max_norm / (norm + 1e-6)) with *norm (device, out)
+ * the norm over the step's gradients, `work` as for dr_grad_norm; a step whose
+ * norm is not finite changes nothing but *norm.  max_norm == 0: coef = 1, norm
+ * and work may be NULL.
+ * state_bits = 8: m is rounded to nearest.  sqrt(v) is rounded to one of its two
+ * neighbours, to the upper one with the probability of its distance from the
+ * lower one: v moves by a factor 1 - beta2 a step, far less than half a code,
+ * and rounding to nearest would hold it where it is.  The 16 random bits of an
+ * element are a fixed function of (seed, t, element).  sqrt(v) > 0 is stored as
+ * 2^-9 * scale at least.
+ * ticket: device uint32, 0 before the first step that uses it, and 0 again
+ * after each; steps that may overlap on the GPU need tickets of their own.
+ * Tensors must not overlap.  `tensors` is a host array, read before the call
+ * returns; the step reads nothing back and can be captured in a CUDA graph, a
+ * replay being the next step. */
+DR_API dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* tensors, int count, double lr,
+                        const float* lr_device, double beta1, double beta2, double eps,
+                        int state_bits, double max_norm, float* norm, void* work,
+                        uint32_t* ticket);
+
 #ifdef __cplusplus
 }
 #endif

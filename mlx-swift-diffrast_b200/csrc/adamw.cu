@@ -1,0 +1,435 @@
+// adamw.cu — the AdamW step over many tensors, with states in 32 or in 8 bits.
+//
+//   g = coef grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Every operation on elements is a separate IEEE round-to-nearest step in
+// float, so a step is the same bit for bit as an unfused evaluation.  The
+// factors in t are formed in double on the device from each tensor's clock
+// (t, b1^t, b2^t), which the step itself advances: nothing in a captured step
+// is fixed to the t of its capture.
+#include <new>
+
+#include "optim_common.cuh"
+
+namespace dr {
+namespace {
+
+struct AdamEntry {
+  void* param;
+  const void* grad;
+  float* master;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  double* clock;
+  int64_t n;
+  double lr_ratio, weight_decay;
+  uint32_t seed;
+  unsigned first_chunk;
+};
+
+struct AdamHyper {
+  double lr, beta1, beta2, max_norm;
+  const float* lr_device;
+  float eps;
+  const double* part;  // partial sums of the norm's squares; nullptr without clipping
+  int parts;
+  float* norm;
+  uint32_t* ticket;
+};
+
+// The list is a kernel parameter (see gradnorm.cu).
+template <int CAP>
+struct AdamTable {
+  AdamEntry t[CAP];
+  AdamHyper h;
+  int count;
+  unsigned chunks;
+};
+constexpr int kSmall = 32, kLarge = 320;
+static_assert(sizeof(AdamTable<kSmall>) <= 4096 && sizeof(AdamTable<kLarge>) <= 32764, "kernel parameters");
+
+// What a step's elements share: for tensor e at its step t.
+struct AdamFactors {
+  float decay;     // 1 - lr wd
+  float step;      // lr / (1 - b1^t)
+  float inv_sqrt;  // 1 / sqrt(1 - b2^t)
+  uint32_t key;    // of the random bits
+};
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+  // Two rounds of xor-shift and multiplication by an odd number (the first 32
+  // bits behind the point of sqrt 2 and sqrt 3): each input bit flips each
+  // output bit with probability 0.500 +- 0.004.
+  x = (x ^ (x >> 16)) * 0x6A09E667u;
+  x = (x ^ (x >> 15)) * 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const AdamHyper& h) {
+  const double t = e.clock[0] + 1.0, b1t = e.clock[1] * h.beta1, b2t = e.clock[2] * h.beta2;
+  const double lr = (h.lr_device ? (double)*h.lr_device : h.lr) * e.lr_ratio;
+  AdamFactors f;
+  f.decay = (float)(1.0 - lr * e.weight_decay);
+  f.step = (float)(lr / (1.0 - b1t));
+  f.inv_sqrt = (float)(1.0 / sqrt(1.0 - b2t));
+  f.key = mix(mix((uint32_t)(long long)t) ^ e.seed);
+  return f;
+}
+
+struct Betas {
+  float b1, b2, one_m_b1, one_m_b2;
+};
+
+__device__ __forceinline__ float next_m(const Betas& b, float m, float g) {
+  return __fadd_rn(__fmul_rn(m, b.b1), __fmul_rn(g, b.one_m_b1));
+}
+__device__ __forceinline__ float next_v(const Betas& b, float v, float g) {
+  return __fadd_rn(__fmul_rn(v, b.b2), __fmul_rn(__fmul_rn(g, g), b.one_m_b2));
+}
+__device__ __forceinline__ float next_p(const AdamFactors& f, float eps, float p, float m, float r) {
+  const float denom = __fadd_rn(__fmul_rn(r, f.inv_sqrt), eps);
+  return __fsub_rn(__fmul_rn(p, f.decay), __fdiv_rn(__fmul_rn(m, f.step), denom));
+}
+
+// One thread's kOptVec elements, loaded and stored whole where they are inside
+// the tensor and every pointer is aligned, else one by one.
+template <typename T>
+__device__ __forceinline__ void load_n(const T* p, bool whole, int valid, float (&x)[kOptVec]) {
+  if (whole) load_vec(p, x);
+  else load_some(p, valid, x);
+}
+template <typename T>
+__device__ __forceinline__ void store_n(T* p, bool whole, int valid, const float (&x)[kOptVec]) {
+  if (whole) store_vec(p, x);
+  else store_some(p, valid, x);
+}
+
+template <typename P, typename G, bool MASTER>
+__device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
+                                         float coef, int64_t at) {
+  const int64_t left = e.n - at;
+  if (left <= 0) return;
+  const int valid = (int)min((int64_t)kOptVec, left);
+  P* p = (P*)e.param + at;
+  const G* g = (const G*)e.grad + at;
+  float* w = e.master + at;
+  float *m = (float*)e.m + at, *v = (float*)e.v + at;
+  const bool whole = valid == kOptVec && (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v |
+                                           (MASTER ? (uintptr_t)w : 0)) & 15) == 0;
+  float xp[kOptVec], xg[kOptVec], xm[kOptVec], xv[kOptVec];
+  if (MASTER) load_n(w, whole, valid, xp);
+  else load_n(p, whole, valid, xp);
+  load_n(g, whole, valid, xg);
+  load_n(m, whole, valid, xm);
+  load_n(v, whole, valid, xv);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) {
+    const float gi = __fmul_rn(xg[i], coef);
+    xm[i] = next_m(b, xm[i], gi);
+    xv[i] = next_v(b, xv[i], gi);
+    xp[i] = next_p(f, eps, xp[i], xm[i], __fsqrt_rn(xv[i]));
+  }
+  store_n(m, whole, valid, xm);
+  store_n(v, whole, valid, xv);
+  if (MASTER) store_n(w, whole, valid, xp);
+  store_n(p, whole, valid, xp);
+}
+
+// 8-bit states: a warp holds a block of 256 elements, eight to a lane.
+constexpr int kStateBlock = 256;
+static_assert(kStateBlock == 32 * kOptVec && kOptChunk % kStateBlock == 0, "one block of states to a warp");
+constexpr float kMaxCode = 448.0f;  // e4m3's largest
+
+__device__ __forceinline__ void codes_to_float(uint2 c, float (&x)[kOptVec]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned short two = (unsigned short)((i < 2 ? c.x : c.y) >> (16 * (i & 1)));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));  // exact
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+__device__ __forceinline__ uint2 float_to_codes(const float (&x)[kOptVec]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    unsigned short lo, hi;  // saturating at +-448, to nearest even; a pair's first element in the low byte
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[4 * i + 1]), "f"(x[4 * i]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[4 * i + 3]), "f"(x[4 * i + 2]));
+    w[i] = (uint32_t)lo | ((uint32_t)hi << 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// Scale of a block and the factor that takes its values to codes.  Below
+// 2^-100 the block is zero (the reciprocal of less would overflow); a value
+// that is not finite makes the whole block NaN.
+__device__ __forceinline__ void scale_of(const float (&x)[kOptVec], float& scale, float& inv) {
+  // Magnitudes order as their bits do, NaN above infinity.
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float t = __uint_as_float(top);
+  if (top >= 0x7F800000u) {
+    scale = inv = __uint_as_float(0x7FC00000u);
+  } else if (t < 0x1p-100f) {
+    scale = inv = 0.0f;
+  } else {
+    scale = __fmul_rn(t, 1.0f / kMaxCode);
+    inv = __fdiv_rn(kMaxCode, t);
+  }
+}
+
+// y >= 0 to one of its two neighbours on e4m3's grid: its low 20 bits and the
+// random ones carry into the last kept bit with the probability of y's distance
+// from the lower neighbour.  Below 2^-6 the grid is even (steps of 2^-9), as it
+// is in [2^-6, 2^-5), where 2^-6 is added for the rounding.
+__device__ __forceinline__ float round_stochastic(float y, uint32_t bits16) {
+  if (y > 0.0f) y = fmaxf(y, 0x1p-9f);  // a moment that is not 0 stays so
+  const float low = y < 0x1p-6f ? 0x1p-6f : 0.0f;
+  const uint32_t w = __float_as_uint(__fadd_rn(y, low)) + (bits16 * 16u + 8u);
+  return fminf(__fsub_rn(__uint_as_float(w & 0xFFF00000u), low), kMaxCode);
+}
+
+template <typename P, typename G, bool MASTER>
+__device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
+                                        float coef, int64_t at) {
+  const int64_t left = e.n - at;
+  const int lane = threadIdx.x & 31;
+  if (left + lane * kOptVec <= 0) return;  // nothing of this block of states is in the tensor: the whole warp leaves
+  const int valid = (int)max((int64_t)0, min((int64_t)kOptVec, left));
+  const int64_t block = at / kStateBlock;
+  P* p = (P*)e.param + at;
+  const G* g = (const G*)e.grad + at;
+  float* w = e.master + at;
+  uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
+  const bool whole = valid == kOptVec &&
+                     (((uintptr_t)p | (uintptr_t)g | (MASTER ? (uintptr_t)w : 0)) & 15) == 0 &&
+                     (((uintptr_t)m | (uintptr_t)v) & 7) == 0;
+  float xp[kOptVec], xg[kOptVec], xm[kOptVec], xr[kOptVec];
+  uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
+  if (whole) {
+    cm = *reinterpret_cast<const uint2*>(m);
+    cr = *reinterpret_cast<const uint2*>(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kOptVec; ++i) {
+      if (i < valid) {
+        (i < 4 ? cm.x : cm.y) |= (uint32_t)m[i] << (8 * (i & 3));
+        (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
+      }
+    }
+  }
+  if (MASTER) load_n(w, whole, valid, xp);
+  else load_n(p, whole, valid, xp);
+  load_n(g, whole, valid, xg);
+  const float sm = e.m_scale[block], sr = e.v_scale[block];
+  codes_to_float(cm, xm);
+  codes_to_float(cr, xr);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) {
+    const float gi = __fmul_rn(xg[i], coef);
+    xm[i] = next_m(b, __fmul_rn(xm[i], sm), gi);
+    const float r = __fmul_rn(xr[i], sr);
+    xr[i] = __fsqrt_rn(next_v(b, __fmul_rn(r, r), gi));
+    xp[i] = next_p(f, eps, xp[i], xm[i], xr[i]);
+    if (i >= valid) xm[i] = xr[i] = 0.0f;  // a block of NaN must not reach its scale from behind the tensor
+  }
+  if (MASTER) store_n(w, whole, valid, xp);
+  store_n(p, whole, valid, xp);
+  float m_scale, m_inv, r_scale, r_inv;
+  scale_of(xm, m_scale, m_inv);
+  scale_of(xr, r_scale, r_inv);
+  const uint32_t key = mix(f.key + (uint32_t)block);
+#pragma unroll
+  for (int i = 0; i < kOptVec; i += 2) {
+    const uint32_t word = mix(key + (uint32_t)(lane * (kOptVec / 2) + i / 2) * 0x9E3779B9u);
+    xm[i] = __fmul_rn(xm[i], m_inv);
+    xm[i + 1] = __fmul_rn(xm[i + 1], m_inv);
+    xr[i] = round_stochastic(__fmul_rn(xr[i], r_inv), word & 0xFFFFu);
+    xr[i + 1] = round_stochastic(__fmul_rn(xr[i + 1], r_inv), word >> 16);
+  }
+  cm = float_to_codes(xm);
+  cr = float_to_codes(xr);
+  if (whole) {
+    *reinterpret_cast<uint2*>(m) = cm;
+    *reinterpret_cast<uint2*>(v) = cr;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kOptVec; ++i) {
+      if (i < valid) {
+        m[i] = (uint8_t)((i < 4 ? cm.x : cm.y) >> (8 * (i & 3)));
+        v[i] = (uint8_t)((i < 4 ? cr.x : cr.y) >> (8 * (i & 3)));
+      }
+    }
+  }
+  if (lane == 0) {
+    e.m_scale[block] = m_scale;
+    e.v_scale[block] = r_scale;
+  }
+}
+
+template <typename P, typename G, bool MASTER, int BITS, int CAP>
+__global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ AdamTable<CAP> tab) {
+  __shared__ AdamFactors s_factors;
+  const AdamHyper& h = tab.h;
+  float coef = 1.0f;
+  bool take = true;
+  if (h.part) {
+    const double norm = norm_of(h.part, h.parts);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
+    coef = clip_factor(norm, h.max_norm);
+    take = isfinite(norm);  // the same in every block
+  }
+  if (!take) return;
+  const Betas b = {(float)h.beta1, (float)h.beta2, (float)(1.0 - h.beta1), (float)(1.0 - h.beta2)};
+  int last = -1;
+  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    const int i = tensor_of(tab.t, tab.count, c);
+    const AdamEntry& e = tab.t[i];
+    if (i != last) {
+      __syncthreads();
+      if (threadIdx.x == 0) s_factors = factors_of(e, h);
+      __syncthreads();
+      last = i;
+    }
+    const AdamFactors f = s_factors;
+    const int64_t at = (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
+    if (BITS == 32) update32<P, G, MASTER>(e, f, b, h.eps, coef, at);
+    else update8<P, G, MASTER>(e, f, b, h.eps, coef, at);
+  }
+  // The last block to come here has every other block's reads of the clocks
+  // behind it: it advances them, and leaves the ticket as it found it.
+  __shared__ bool s_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(h.ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < tab.count; i += kOptThreads) {
+    double* k = tab.t[i].clock;
+    k[0] += 1.0;
+    k[1] *= h.beta1;
+    k[2] *= h.beta2;
+  }
+  if (threadIdx.x == 0) *h.ticket = 0;
+}
+
+// One launch for the tensors of one combination of types, CAP at a time.
+template <typename P, typename G, bool MASTER, int BITS, int CAP>
+dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyper& h, int pt, int gt) {
+  for (int i = 0; i < count;) {
+    AdamTable<CAP> tab;
+    int64_t chunks = 0;
+    tab.count = 0;
+    tab.h = h;
+    for (; i < count && tab.count < CAP; ++i) {
+      const dr_adamw_tensor& x = t[i];
+      if (x.n == 0 || x.param_type != pt || x.grad_type != gt || (x.master != nullptr) != MASTER) continue;
+      tab.t[tab.count++] = {x.param,   x.grad, x.master, x.m,        x.v,            x.m_scale, x.v_scale,
+                            x.clock,   x.n,    x.lr_ratio, x.weight_decay, x.seed, (unsigned)chunks};
+      chunks += opt_chunks(x.n);
+    }
+    if (tab.count == 0) break;
+    tab.chunks = (unsigned)chunks;
+    const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 8);
+    DR_TB(ctx);
+    k_adamw<P, G, MASTER, BITS, CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+    DR_LAUNCHED(ctx, BITS == 32 ? "adamw" : "adamw8");
+  }
+  return DR_OK;
+}
+
+template <typename P, typename G, bool MASTER>
+dr_status launch_types(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyper& h, int bits, int pt,
+                       int gt) {
+  int members = 0;
+  for (int i = 0; i < count; ++i)
+    members += t[i].n != 0 && t[i].param_type == pt && t[i].grad_type == gt && (t[i].master != nullptr) == MASTER;
+  if (members == 0) return DR_OK;
+  if (members <= kSmall)
+    return bits == 32 ? launch<P, G, MASTER, 32, kSmall>(ctx, t, count, h, pt, gt)
+                      : launch<P, G, MASTER, 8, kSmall>(ctx, t, count, h, pt, gt);
+  return bits == 32 ? launch<P, G, MASTER, 32, kLarge>(ctx, t, count, h, pt, gt)
+                    : launch<P, G, MASTER, 8, kLarge>(ctx, t, count, h, pt, gt);
+}
+
+}  // namespace
+}  // namespace dr
+
+using namespace dr;
+
+extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int count, double lr,
+                                   const float* lr_device, double beta1, double beta2, double eps, int state_bits,
+                                   double max_norm, float* norm, void* work, uint32_t* ticket) {
+  DR_ENTER(ctx);
+  DR_REQUIRE(ctx, count >= 0 && (count == 0 || t), "adamw: null list or count < 0");
+  DR_REQUIRE(ctx, state_bits == 32 || state_bits == 8, "adamw: state_bits must be 32 or 8");
+  DR_REQUIRE(ctx, ticket, "adamw: ticket is required");
+  DR_REQUIRE(ctx, lr_device || (lr >= 0.0 && lr < 1e30), "adamw: lr must be finite and not negative");
+  DR_REQUIRE(ctx, beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: betas must be in [0, 1)");
+  DR_REQUIRE(ctx, (float)eps > 0.0f && eps < 1e30, "adamw: eps must be positive (in float) and finite");
+  DR_REQUIRE(ctx, max_norm >= 0.0 && max_norm < 1e300, "adamw: max_norm must be finite and not negative");
+  DR_REQUIRE(ctx, max_norm == 0.0 || (norm && work && ((uintptr_t)work & 7) == 0),
+             "adamw: clipping needs norm and an 8-byte aligned work");
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    const dr_adamw_tensor& x = t[i];
+    DR_REQUIRE(ctx, x.n >= 0 && x.n < kOptMostElements && (chunks += opt_chunks(x.n)) < INT32_MAX,
+               "adamw: tensor %d: n < 0, or too many elements", i);
+    DR_REQUIRE(ctx, x.n == 0 || (x.param && x.grad && x.m && x.v && x.clock), "adamw: tensor %d: null pointer", i);
+    DR_REQUIRE(ctx, x.n == 0 || state_bits == 32 || (x.m_scale && x.v_scale), "adamw: tensor %d: scales are required",
+               i);
+    DR_REQUIRE(ctx, valid_type(x.param_type) && valid_type(x.grad_type) &&
+                        (x.grad_type == x.param_type || x.grad_type == DR_F32 || x.param_type == DR_F32),
+               "adamw: tensor %d: types %d and %d", i, x.param_type, x.grad_type);
+    DR_REQUIRE(ctx, !x.master || x.param_type != DR_F32, "adamw: tensor %d: fp32 has no master weights", i);
+    const uintptr_t ps = x.param_type == DR_F32 ? 4 : 2, gs = x.grad_type == DR_F32 ? 4 : 2;
+    const uintptr_t ss = state_bits == 32 ? 4 : 1;
+    DR_REQUIRE(ctx, (uintptr_t)x.param % ps == 0 && (uintptr_t)x.grad % gs == 0 && (uintptr_t)x.m % ss == 0 &&
+                        (uintptr_t)x.v % ss == 0 && (uintptr_t)x.master % 4 == 0 && (uintptr_t)x.m_scale % 4 == 0 &&
+                        (uintptr_t)x.v_scale % 4 == 0 && (uintptr_t)x.clock % 8 == 0,
+               "adamw: tensor %d: misaligned pointer", i);
+    DR_REQUIRE(ctx, x.lr_ratio >= 0.0 && x.lr_ratio < 1e30 && x.weight_decay >= 0.0 && x.weight_decay < 1e30,
+               "adamw: tensor %d: lr_ratio and weight_decay must be finite and not negative", i);
+  }
+  AdamHyper h = {lr, beta1, beta2, max_norm, lr_device, (float)eps, nullptr, 0, norm, ticket};
+  if (max_norm > 0.0) {
+    dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
+    if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);
+    for (int i = 0; i < count; ++i) g[i] = {const_cast<void*>(t[i].grad), t[i].n, t[i].grad_type, 0};
+    const dr_status st = grad_norm_parts(ctx, g, count, (double*)work, &h.parts);
+    delete[] g;
+    if (st != DR_OK) return st;
+    h.part = (const double*)work;
+    if (h.parts == 0) return grad_norm_finish(ctx, (const double*)work, 0, norm);
+  }
+#define DR_ADAMW(P, G, MASTER, PT, GT)                                                                  \
+  do {                                                                                                  \
+    const dr_status st = launch_types<P, G, MASTER>(ctx, t, count, h, state_bits, PT, GT);              \
+    if (st != DR_OK) return st;                                                                         \
+  } while (0)
+  DR_ADAMW(float, float, false, DR_F32, DR_F32);
+  DR_ADAMW(float, __nv_bfloat16, false, DR_F32, DR_BF16);
+  DR_ADAMW(float, __half, false, DR_F32, DR_F16);
+  DR_ADAMW(__nv_bfloat16, __nv_bfloat16, false, DR_BF16, DR_BF16);
+  DR_ADAMW(__nv_bfloat16, float, false, DR_BF16, DR_F32);
+  DR_ADAMW(__nv_bfloat16, __nv_bfloat16, true, DR_BF16, DR_BF16);
+  DR_ADAMW(__nv_bfloat16, float, true, DR_BF16, DR_F32);
+  DR_ADAMW(__half, __half, false, DR_F16, DR_F16);
+  DR_ADAMW(__half, float, false, DR_F16, DR_F32);
+  DR_ADAMW(__half, __half, true, DR_F16, DR_F16);
+  DR_ADAMW(__half, float, true, DR_F16, DR_F32);
+#undef DR_ADAMW
+  return DR_OK;
+}

@@ -1,0 +1,126 @@
+// optim_common.cuh — what the many-tensor optimizer kernels share: element
+// types, the split of a list of tensors into chunks, and the gradient norm's
+// partial sums.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace dr {
+
+constexpr int kOptThreads = 256;
+constexpr int kOptVec = 8;                          // consecutive elements of one thread
+constexpr int kOptChunk = kOptThreads * kOptVec;    // elements a block handles at once
+
+// Elements of one thread, widened to float.  The 16-bit types widen exactly.
+template <typename T>
+__device__ __forceinline__ float widen(T x);
+template <>
+__device__ __forceinline__ float widen(float x) { return x; }
+template <>
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+
+// Rounding to nearest even: parameters and gradients are what a user stores in
+// 16 bits; everything in between stays in float.
+template <typename T>
+__device__ __forceinline__ T narrow(float x);
+template <>
+__device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
+
+// kOptVec consecutive elements at a 16-byte aligned address.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[kOptVec]) {
+  constexpr int kWords = kOptVec * sizeof(T) / 16;
+  uint4 w[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) x[i] = widen(e[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[kOptVec]) {
+  constexpr int kWords = kOptVec * sizeof(T) / 16;
+  uint4 w[kWords];
+  T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) e[i] = narrow<T>(x[i]);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+}
+
+// `valid` (0 .. kOptVec) elements at any address of T's alignment; the others are 0.
+template <typename T>
+__device__ __forceinline__ void load_some(const T* p, int valid, float (&x)[kOptVec]) {
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) x[i] = i < valid ? widen(p[i]) : 0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, int valid, const float (&x)[kOptVec]) {
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i)
+    if (i < valid) p[i] = narrow<T>(x[i]);
+}
+
+// A list holds fewer chunks than an int does (4e12 elements), checked at the entries.
+constexpr int64_t kOptMostElements = (int64_t)INT32_MAX * kOptChunk;
+inline int64_t opt_chunks(int64_t n) { return (n + kOptChunk - 1) / kOptChunk; }
+
+// The tensor of a list that chunk c belongs to: the last whose first chunk is
+// <= c.  Tensors without elements are not in the list, so it is the one.
+template <typename Entry>
+__device__ __forceinline__ int tensor_of(const Entry* t, int count, unsigned c) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t[mid].first_chunk <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Sum over the block in a fixed order; every thread gets it.  kOptThreads threads.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double s_warp[kOptThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();  // s_warp may still be read from an earlier call
+  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kOptThreads / 32; ++i) s += s_warp[i];
+  return s;
+}
+
+// The norm that `count` partial sums of squares give: the same value in every
+// block that asks, whatever its place.
+__device__ __forceinline__ double norm_of(const double* part, int count) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += kOptThreads) s += part[i];
+  return sqrt(block_sum(s));
+}
+
+// min(1, max_norm / (norm + 1e-6)); a NaN stays one.
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+  const double c = max_norm / (norm + 1e-6);
+  return c >= 1.0 ? 1.0f : (float)c;
+}
+
+bool valid_type(int type);
+// Launches the partial sums of squares of a list; *parts of them lie in `work`.
+dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts);
+// *norm = the norm that the partial sums give.
+dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* norm);
+
+}  // namespace dr

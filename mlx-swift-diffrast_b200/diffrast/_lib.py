@@ -22,6 +22,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 I64 = ctypes.c_int64
 F = ctypes.c_float
+D = ctypes.c_double
 
 # name -> (restype, argtypes), mirroring include/diffrast.h
 SIGNATURES = {
@@ -72,6 +73,10 @@ SIGNATURES = {
     "dr_mse_fwd_bwd": (I, [P, P, P, I64, F, P, P, I]),
     "dr_mse_bwd": (I, [P, P, P, I64, F, P, P]),
     "dr_adam_step": (I, [P, P, P, P, P, P, I64, F, F, F, F, F, F]),
+    "dr_grad_norm_work_bytes": (ctypes.c_size_t, [P, I]),
+    "dr_grad_norm": (I, [P, P, I, P, P]),
+    "dr_clip_grad_norm": (I, [P, P, I, D, P, P]),
+    "dr_adamw_step": (I, [P, P, I, D, P, D, D, D, I, D, P, P, P]),
 }
 
 _lib = None
