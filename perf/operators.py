@@ -133,6 +133,13 @@ def work(case):
     return {"bytes": n * (weights + g + state) + 16 * blocks, "flops": flops * n}
 
 
+def _package():
+    if "diffrast.optim" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.getcwd(), "mlx-swift-diffrast_b200"))
+    from diffrast import optim
+    return optim
+
+
 def prepare(case, seed):
     dev = torch.device("cuda")
     gen = torch.Generator(device=dev)
@@ -188,9 +195,7 @@ def prepare(case, seed):
                 st[key] = torch.where(floor, torch.full_like(x, 2.0 ** -9), st[key].float()).to(torch.float8_e4m3fn)
     if own:
         # The optimizer that the user's program keeps, with the state of a run in progress.
-        if "mlx-swift-diffrast_b200" not in sys.path:
-            sys.path.insert(0, os.path.join(os.getcwd(), "mlx-swift-diffrast_b200"))
-        from diffrast import optim
+        optim = _package()
         opt = optim.AdamW(st["params"], learning_rate=LR, beta1=B1, beta2=B2, eps=EPS, weight_decay=WD,
                           state_bits=case["bits"], master_weights=case["master"],
                           max_grad_norm=case["max_norm"] or None, seed=SEED)
@@ -216,9 +221,7 @@ def run(st):
     if own:
         if case["op"] == "adamw":
             return _outputs(st, st["opt"].step(st["grads"]))
-        if "mlx-swift-diffrast_b200" not in sys.path:
-            sys.path.insert(0, os.path.join(os.getcwd(), "mlx-swift-diffrast_b200"))
-        from diffrast import optim
+        optim = _package()
         if case["op"] == "grad_norm":
             return {"norm": optim.grad_norm(st["grads"])}
         return {"norm": optim.clip_grad_norm_(st["grads"], case["max_norm"]), "g": st["g"]}
