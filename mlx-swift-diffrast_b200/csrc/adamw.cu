@@ -8,6 +8,7 @@
 // factors in t are formed in double on the device from each tensor's clock
 // (t, b1^t, b2^t), which the step itself advances: nothing in a captured step
 // is fixed to the t of its capture.
+#include <cmath>
 #include <new>
 
 #include "optim_common.cuh"
@@ -28,6 +29,14 @@ struct AdamEntry {
   double lr_ratio, weight_decay;
   uint32_t seed;
   unsigned first_chunk;
+  unsigned end_chunk;
+  int aligned;  // whether every vector of the tensor may be accessed whole
+};
+
+// beta1, beta2, what they leave of 1, and the roots of beta2 and of its rest.
+struct Betas {
+  float b1, b2, one_m_b1, one_m_b2;
+  float root_b2, root_one_m_b2;
 };
 
 struct AdamHyper {
@@ -38,6 +47,7 @@ struct AdamHyper {
   int parts;
   float* norm;
   uint32_t* ticket;
+  Betas betas;
 };
 
 // The list is a kernel parameter (see gradnorm.cu).
@@ -48,7 +58,7 @@ struct AdamTable {
   int count;
   unsigned chunks;
 };
-constexpr int kSmall = 32, kLarge = 320;
+constexpr int kSmall = 32, kLarge = 304;
 static_assert(sizeof(AdamTable<kSmall>) <= 4096 && sizeof(AdamTable<kLarge>) <= 32764, "kernel parameters");
 
 // What a step's elements share: for tensor e at its step t.
@@ -78,10 +88,6 @@ __device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const Adam
   f.key = mix(mix((uint32_t)(long long)t) ^ e.seed);
   return f;
 }
-
-struct Betas {
-  float b1, b2, one_m_b1, one_m_b2;
-};
 
 __device__ __forceinline__ float next_m(const Betas& b, float m, float g) {
   return __fadd_rn(__fmul_rn(m, b.b1), __fmul_rn(g, b.one_m_b1));
@@ -117,8 +123,7 @@ __device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& 
   const G* g = (const G*)e.grad + at;
   float* w = e.master + at;
   float *m = (float*)e.m + at, *v = (float*)e.v + at;
-  const bool whole = valid == kOptVec && (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v |
-                                           (MASTER ? (uintptr_t)w : 0)) & 15) == 0;
+  const bool whole = e.aligned && valid == kOptVec;
   float xp[kOptVec], xg[kOptVec], xm[kOptVec], xv[kOptVec];
   if (MASTER) load_n(w, whole, valid, xp);
   else load_n(p, whole, valid, xp);
@@ -167,36 +172,74 @@ __device__ __forceinline__ uint2 float_to_codes(const float (&x)[kOptVec]) {
   return make_uint2(w[0], w[1]);
 }
 
-// Scale of a block and the factor that takes its values to codes.  Below
-// 2^-100 the block is zero (the reciprocal of less would overflow); a value
-// that is not finite makes the whole block NaN.
-__device__ __forceinline__ void scale_of(const float (&x)[kOptVec], float& scale, float& inv) {
-  // Magnitudes order as their bits do, NaN above infinity.
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kOptVec; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  top = __reduce_max_sync(0xffffffffu, top);
-  const float t = __uint_as_float(top);
-  if (top >= 0x7F800000u) {
-    scale = inv = __uint_as_float(0x7FC00000u);
-  } else if (t < 0x1p-100f) {
-    scale = inv = 0.0f;
-  } else {
-    scale = __fmul_rn(t, 1.0f / kMaxCode);
-    inv = __fdiv_rn(kMaxCode, t);
-  }
+// Two floats in a register pair: one instruction for both, each rounded as
+// the single one is.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ Two both(float x) { return two(x, x); }
+__device__ __forceinline__ float2 apart(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// To 2^-23 relative; arguments below 2^-126 count as 0.
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// To one unit in the last place, for a normal argument and result.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
 }
 
-// y >= 0 to one of its two neighbours on e4m3's grid: its low 20 bits and the
-// random ones carry into the last kept bit with the probability of y's distance
-// from the lower neighbour.  Below 2^-6 the grid is even (steps of 2^-9), as it
-// is in [2^-6, 2^-5), where 2^-6 is added for the rounding.
-__device__ __forceinline__ float round_stochastic(float y, uint32_t bits16) {
-  if (y > 0.0f) y = fmaxf(y, 0x1p-9f);  // a moment that is not 0 stays so
-  const float low = y < 0x1p-6f ? 0x1p-6f : 0.0f;
-  const uint32_t w = __float_as_uint(__fadd_rn(y, low)) + (bits16 * 16u + 8u);
-  return fminf(__fsub_rn(__uint_as_float(w & 0xFFF00000u), low), kMaxCode);
+// Scale of a block, from each lane's largest magnitude, and the factor that
+// takes its values to codes.  Below 2^-100 the block is zero; a value that is
+// not finite makes the whole block NaN.
+__device__ __forceinline__ void scale_of(float lane_top, float& scale, float& inv) {
+  // Magnitudes order as their bits do, NaN above infinity.
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(lane_top));
+  const float t = __uint_as_float(top);
+  scale = __fmul_rn(t, 1.0f / kMaxCode);
+  inv = rcp_fast(scale);
+  if (t < 0x1p-100f) scale = inv = 0.0f;
+  if (top >= 0x7F800000u) scale = inv = __uint_as_float(0x7FC00000u);
 }
+
+// The code of a value r >= 0, given z = 2^-120 (r / scale): e4m3's grid is that
+// of z's bits above the lowest 20, its small evenly spaced values lying where
+// float's are.  The low bits and the random ones carry into the last kept bit
+// with the probability of z's distance from the lower neighbour.  What is not 0
+// becomes code 1 at least, and the largest code is 0x7E.
+__device__ __forceinline__ uint32_t round_stochastic(float z, float r, uint32_t bits16) {
+  const uint32_t w = max(__float_as_uint(z), min(__float_as_uint(r), 1u << 20));
+  return min(w + bits16 * 16u + 8u, 0x7EFFFFFu) >> 20;
+}
+
+constexpr uint32_t kGolden = 0x9E3779B9u;
 
 template <typename P, typename G, bool MASTER>
 __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
@@ -210,9 +253,7 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   const G* g = (const G*)e.grad + at;
   float* w = e.master + at;
   uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
-  const bool whole = valid == kOptVec &&
-                     (((uintptr_t)p | (uintptr_t)g | (MASTER ? (uintptr_t)w : 0)) & 15) == 0 &&
-                     (((uintptr_t)m | (uintptr_t)v) & 7) == 0;
+  const bool whole = e.aligned && valid == kOptVec;
   float xp[kOptVec], xg[kOptVec], xm[kOptVec], xr[kOptVec];
   uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
   if (whole) {
@@ -230,34 +271,54 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   if (MASTER) load_n(w, whole, valid, xp);
   else load_n(p, whole, valid, xp);
   load_n(g, whole, valid, xg);
-  const float sm = e.m_scale[block], sr = e.v_scale[block];
+  const Two sm = both(__fmul_rn(e.m_scale[block], b.b1)), sr = both(__fmul_rn(e.v_scale[block], b.root_b2));
   codes_to_float(cm, xm);
   codes_to_float(cr, xr);
+  const Two kc = both(coef), km = both(b.one_m_b1), kr = both(b.root_one_m_b2), ki = both(f.inv_sqrt), ke = both(eps),
+            ks = both(-f.step), kd = both(f.decay);
+  float m_top = 0.0f, r_top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kOptVec; ++i) {
-    const float gi = __fmul_rn(xg[i], coef);
-    xm[i] = next_m(b, __fmul_rn(xm[i], sm), gi);
-    const float r = __fmul_rn(xr[i], sr);
-    xr[i] = __fsqrt_rn(next_v(b, __fmul_rn(r, r), gi));
-    xp[i] = next_p(f, eps, xp[i], xm[i], xr[i]);
-    if (i >= valid) xm[i] = xr[i] = 0.0f;  // a block of NaN must not reach its scale from behind the tensor
+  for (int i = 0; i < kOptVec; i += 2) {
+    const Two gi = two(xg[i], xg[i + 1]) * kc;
+    const Two mi = fma2(two(xm[i], xm[i + 1]), sm, gi * km);
+    // v = (sqrt(b2) r)^2 + (sqrt(1 - b2) g)^2
+    const Two a = two(xr[i], xr[i + 1]) * sr, c = gi * kr;
+    const float2 v2 = apart(fma2(a, a, c * c));
+    const float2 r2 = make_float2(sqrt_fast(v2.x), sqrt_fast(v2.y));
+    const float2 d = apart(fma2(two(r2.x, r2.y), ki, ke));
+    const float2 np = apart(fma2(mi * ks, two(rcp_fast(d.x), rcp_fast(d.y)), two(xp[i], xp[i + 1]) * kd));
+    const float2 nm = apart(mi);
+    xp[i] = np.x;
+    xp[i + 1] = np.y;
+    // Behind the tensor's end there is nothing: a block of NaN must not reach its scale from there.
+    xm[i] = i < valid ? nm.x : 0.0f;
+    xm[i + 1] = i + 1 < valid ? nm.y : 0.0f;
+    xr[i] = i < valid ? r2.x : 0.0f;
+    xr[i + 1] = i + 1 < valid ? r2.y : 0.0f;
+    m_top = max_nan(max_nan(m_top, fabsf(xm[i])), fabsf(xm[i + 1]));
+    r_top = max_nan(max_nan(r_top, xr[i]), xr[i + 1]);
   }
   if (MASTER) store_n(w, whole, valid, xp);
   store_n(p, whole, valid, xp);
   float m_scale, m_inv, r_scale, r_inv;
-  scale_of(xm, m_scale, m_inv);
-  scale_of(xr, r_scale, r_inv);
-  const uint32_t key = mix(f.key + (uint32_t)block);
+  scale_of(m_top, m_scale, m_inv);
+  scale_of(r_top, r_scale, r_inv);
+  const uint32_t key = mix(f.key + (uint32_t)block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
+  const Two im = both(m_inv), ir = both(r_inv), grid = both(0x1p-120f);
+  uint32_t code[kOptVec];
 #pragma unroll
   for (int i = 0; i < kOptVec; i += 2) {
-    const uint32_t word = mix(key + (uint32_t)(lane * (kOptVec / 2) + i / 2) * 0x9E3779B9u);
-    xm[i] = __fmul_rn(xm[i], m_inv);
-    xm[i + 1] = __fmul_rn(xm[i + 1], m_inv);
-    xr[i] = round_stochastic(__fmul_rn(xr[i], r_inv), word & 0xFFFFu);
-    xr[i + 1] = round_stochastic(__fmul_rn(xr[i + 1], r_inv), word >> 16);
+    const float2 qm = apart(two(xm[i], xm[i + 1]) * im);
+    const float2 qr = apart(two(xr[i], xr[i + 1]) * ir * grid);
+    const uint32_t word = mix(key + i / 2 * kGolden);
+    code[i] = round_stochastic(qr.x, xr[i], word & 0xFFFFu);
+    code[i + 1] = round_stochastic(qr.y, xr[i + 1], word >> 16);
+    xm[i] = qm.x;
+    xm[i + 1] = qm.y;
   }
   cm = float_to_codes(xm);
-  cr = float_to_codes(xr);
+  cr = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                  code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
   if (whole) {
     *reinterpret_cast<uint2*>(m) = cm;
     *reinterpret_cast<uint2*>(v) = cr;
@@ -289,10 +350,10 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
     take = isfinite(norm);  // the same in every block
   }
   if (!take) return;
-  const Betas b = {(float)h.beta1, (float)h.beta2, (float)(1.0 - h.beta1), (float)(1.0 - h.beta2)};
-  int last = -1;
+  const Betas b = h.betas;
+  int i = tensor_of(tab.t, tab.count, blockIdx.x), last = -1;
   for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    const int i = tensor_of(tab.t, tab.count, c);
+    while (c >= tab.t[i].end_chunk) ++i;
     const AdamEntry& e = tab.t[i];
     if (i != last) {
       __syncthreads();
@@ -336,8 +397,12 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     for (; i < count && tab.count < CAP; ++i) {
       const dr_adamw_tensor& x = t[i];
       if (x.n == 0 || x.param_type != pt || x.grad_type != gt || (x.master != nullptr) != MASTER) continue;
+      const uintptr_t state = (uintptr_t)x.m | (uintptr_t)x.v;
+      const int aligned = (((uintptr_t)x.param | (uintptr_t)x.grad | (uintptr_t)x.master) & 15) == 0 &&
+                          (state & (BITS == 32 ? 15 : 7)) == 0;
       tab.t[tab.count++] = {x.param,   x.grad, x.master, x.m,        x.v,            x.m_scale, x.v_scale,
-                            x.clock,   x.n,    x.lr_ratio, x.weight_decay, x.seed, (unsigned)chunks};
+                            x.clock,   x.n,    x.lr_ratio, x.weight_decay, x.seed, (unsigned)chunks, (unsigned)(chunks + opt_chunks(x.n)),
+                            aligned};
       chunks += opt_chunks(x.n);
     }
     if (tab.count == 0) break;
@@ -378,7 +443,7 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
   DR_REQUIRE(ctx, ticket, "adamw: ticket is required");
   DR_REQUIRE(ctx, lr_device || (lr >= 0.0 && lr < 1e30), "adamw: lr must be finite and not negative");
   DR_REQUIRE(ctx, beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: betas must be in [0, 1)");
-  DR_REQUIRE(ctx, (float)eps > 0.0f && eps < 1e30, "adamw: eps must be positive (in float) and finite");
+  DR_REQUIRE(ctx, eps >= 0x1p-126 && eps < 1e30, "adamw: eps must be at least 2^-126 and finite");
   DR_REQUIRE(ctx, max_norm >= 0.0 && max_norm < 1e300, "adamw: max_norm must be finite and not negative");
   DR_REQUIRE(ctx, max_norm == 0.0 || (norm && work && ((uintptr_t)work & 7) == 0),
              "adamw: clipping needs norm and an 8-byte aligned work");
@@ -403,7 +468,9 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
     DR_REQUIRE(ctx, x.lr_ratio >= 0.0 && x.lr_ratio < 1e30 && x.weight_decay >= 0.0 && x.weight_decay < 1e30,
                "adamw: tensor %d: lr_ratio and weight_decay must be finite and not negative", i);
   }
-  AdamHyper h = {lr, beta1, beta2, max_norm, lr_device, (float)eps, nullptr, 0, norm, ticket};
+  AdamHyper h = {lr, beta1, beta2, max_norm, lr_device, (float)eps, nullptr, 0, norm, ticket,
+                 {(float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)std::sqrt(beta2),
+                  (float)std::sqrt(1.0 - beta2)}};
   if (max_norm > 0.0) {
     dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
     if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);

@@ -205,8 +205,8 @@ class AdamW:
         for name, b in (("beta1", beta1), ("beta2", beta2)):
             if not 0.0 <= float(b) < 1.0:
                 raise ValueError(f"AdamW: {name} must be in [0, 1) (got {b})")
-        if not (np.float32(eps) > 0 and math.isfinite(eps)):
-            raise ValueError(f"AdamW: eps must be positive in float32 and finite (got {eps})")
+        if not 2.0 ** -126 <= float(eps) < 1e30:
+            raise ValueError(f"AdamW: eps must be at least 2^-126 and finite (got {eps})")
         self.beta1, self.beta2, self.eps = float(beta1), float(beta2), float(eps)
         self.state_bits, self.seed = int(state_bits), int(seed)
         self.learning_rate = learning_rate

@@ -14,30 +14,40 @@ def clip_factor(norm, max_norm):
     return min(1.0, max_norm / (norm + 1e-6)) if max_norm else 1.0
 
 
-def step(p, g, m, r, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, wd=1e-2, coef=1.0, clipped=False, dequant=0):
-    """One step t from p, gradient g, first moment m and second moment's root r, all float64.
-    Returns (p, m, v) and their bounds (dp, dm, dv).  dequant: roundings that m and r carry already."""
-    c = 2 if clipped else 0  # the factor's rounding and the product's
+def step(p, g, m, r, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, wd=1e-2, coef=1.0, clipped=False, bits=32):
+    """One step t from p, gradient g, first moment m and second moment's root r, all float64, where m and r are float32
+    values: with 32-bit states m and the rounded root of v, with 8-bit states the rounded products of code and scale.
+    Returns (p, m, v) and their bounds (dp, dm, dv), in units of U (half a step of float32), term by term:
+
+    32 bits.  m: beta's rounding, the product's, the sum's.  v: the same on beta2 v, and v's root, rounded (2 in v), is
+      what is known of it; the square's rounding, the factor's, the product's and the sum's on (1 - beta2) g^2.
+    8 bits.  m: the known m's rounding, beta's, its product's with the scale, the sum's.  v = (root(beta2) r)^2 +
+      (root(1 - beta2) g)^2: the known r's, the root's, its product's with the scale and the product's with the code
+      count twice, the sum's once; of g's term the root's and the product's twice, the square's and the sum's once.
+      sqrt is within two units, one reciprocal within two.
+    Clipping: the factor's rounding and the product's, on g.
+    p: 1 - lr wd and its product; of the update the factor lr / (1 - beta1^t), its product, the factor of r, its
+      product, the sum with eps, the quotient (8 bits: reciprocal, two), what m and r carry; the difference."""
+    c = 2 if clipped else 0
     g = g * coef
     a, b = np.abs(beta1 * m), np.abs((1 - beta1) * g)
     m2 = beta1 * m + (1 - beta1) * g
-    # beta's rounding, the product's, the sum's; the state's own where it was just dequantised
-    dm = U * ((3 + dequant) * a + (3 + c) * b)
     x, y = beta2 * r * r, (1 - beta2) * g * g
     v2 = x + y
-    # a product more (the square) in each term; the root's own roundings count twice in it
-    dv = U * ((4 + 2 * dequant) * x + (4 + 2 * c) * y)
+    if bits == 32:
+        dm, dv, root = U * (3 * a + (3 + c) * b), U * (5 * x + (4 + 2 * c) * y), 1
+    else:
+        dm, dv, root = U * (4 * a + (3 + c) * b), U * (9 * x + (6 + 2 * c) * y), 2
     r2 = np.sqrt(v2)
-    with np.errstate(divide="ignore", invalid="ignore"):
-        dr = np.where(v2 > 0, dv / (2 * np.maximum(r2, 1e-300)), 0.0) + U * r2
-    denom = r2 / np.sqrt(1 - beta2 ** t) + eps
+    dr = np.where(v2 > 0, dv / (2 * np.maximum(r2, 1e-300)), 0.0) + root * U * r2
+    root_c2 = np.sqrt(1 - beta2 ** t)
+    denom = r2 / root_c2 + eps
     step_ = lr / (1 - beta1 ** t)
     upd = step_ * m2 / denom
     p2 = p * (1 - lr * wd) - upd
-    # the factor's rounding and the product's; the quotient's three, the denominator's four and what m and r carry
-    dupd = step_ * dm / denom + np.abs(upd) * (7 * U + dr / np.maximum(r2 + eps * np.sqrt(1 - beta2 ** t), 1e-300))
-    dp = 2 * U * np.abs(p * (1 - lr * wd)) + dupd * (1 + 1e-5)
-    dp = dp + U * np.abs(p2) + 1e-45
+    dupd = step_ * dm / denom + np.abs(upd) * (7 * U + dr / (r2 + eps * root_c2))
+    # second-order terms: every relative error here is below 1e-5
+    dp = (2 * U * np.abs(p * (1 - lr * wd)) + dupd) * (1 + 1e-5) + U * np.abs(p2) + 1e-45
     # Products below the smallest normal number lose up to half of the smallest one, and v and r with them.
     tiny = 2.0 ** -149
     return (p2, m2, v2), (dp, dm + 2 * tiny, dv + 3 * tiny)

@@ -49,7 +49,7 @@ def check_step(opt, before, grads, norm, lr, wd=1e-2, eps=1e-8):
         t = int(t0) + 1
         assert t1 == t and abs(b1t / 0.9 ** t - 1) < 1e-13 and abs(b2t / 0.999 ** t - 1) < 1e-13
         (p2, m2, v2), (dp, dm, dv) = AO.step(p0, f64(g.contiguous()), m0, r0, t, lr, wd=wd, eps=eps, coef=coef,
-                                             clipped=bool(top), dequant=1 if opt.state_bits == 8 else 2)
+                                             clipped=bool(top), bits=opt.state_bits)
         held = "master" in opt.state and opt._half[i]
         weights = f64(opt._flat("master", i)) if held else f64(p)
         if held:
@@ -63,7 +63,7 @@ def check_step(opt, before, grads, norm, lr, wd=1e-2, eps=1e-8):
             assert np.all(np.abs(f64(opt._flat("v", i)) - v2) <= dv)
             continue
         r2 = np.sqrt(v2)
-        for name, x, dx in (("m", m2, dm), ("r", r2, np.where(v2 > 0, dv / np.maximum(2 * r2, 1e-300), 0) + AO.U * r2)):
+        for name, x, dx in (("m", m2, dm), ("r", r2, np.where(v2 > 0, dv / np.maximum(2 * r2, 1e-300), 0) + 2 * AO.U * r2)):
             scale = f64(opt._flat(name + "_scale", i))
             ref = AO.scales(x)
             np.testing.assert_allclose(scale, ref, rtol=2 * AO.U + float(np.max(dx / np.maximum(np.abs(x), 1e-300),
@@ -386,7 +386,7 @@ def test_adamw_ratios_decays_and_a_device_learning_rate(bits):
         for i in range(3):
             p0, m0, r0, t0 = before[i]
             (p2, _, _), (dp, _, _) = AO.step(p0, f64(gs[i]), m0, r0, int(t0) + 1, 0.03125 * 0.5 ** (k + 1) * ratios[i],
-                                             wd=decays[i], dequant=2)
+                                             wd=decays[i], bits=bits)
             assert np.all(np.abs(f64(params[i]) - p2) <= dp)
 
 
