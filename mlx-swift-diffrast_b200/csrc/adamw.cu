@@ -8,8 +8,8 @@
 // factors in t are formed in double on the device from each tensor's clock
 // (t, b1^t, b2^t), which the step itself advances: nothing in a captured step
 // is fixed to the t of its capture.
-#include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "optim_common.cuh"
 
@@ -33,10 +33,9 @@ struct AdamEntry {
   int aligned;  // whether every vector of the tensor may be accessed whole
 };
 
-// beta1, beta2, what they leave of 1, and the roots of beta2 and of its rest.
+// beta1, beta2 and what they leave of 1.
 struct Betas {
   float b1, b2, one_m_b1, one_m_b2;
-  float root_b2, root_one_m_b2;
 };
 
 struct AdamHyper {
@@ -113,6 +112,7 @@ __device__ __forceinline__ void store_n(T* p, bool whole, int valid, const float
   else store_some(p, valid, x);
 }
 
+// 32-bit states: one thread's elements at `at`.
 template <typename P, typename G, bool MASTER>
 __device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
                                          float coef, int64_t at) {
@@ -198,68 +198,123 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-// To 2^-23 relative; arguments below 2^-126 count as 0.
-__device__ __forceinline__ float sqrt_fast(float x) {
-  float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-// To one unit in the last place, for a normal argument and result.
+// The hardware's approximations, within one or two units in the last place.
+__device__ __forceinline__ float rsqrt_fast(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float rcp_fast(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float max_nan(float x, float y) {
+__device__ __forceinline__ float max_nan(float x, float y, float z) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
 
-// Scale of a block, from each lane's largest magnitude, and the factor that
-// takes its values to codes.  Below 2^-100 the block is zero; a value that is
-// not finite makes the whole block NaN.
-__device__ __forceinline__ void scale_of(float lane_top, float& scale, float& inv) {
-  // Magnitudes order as their bits do, NaN above infinity.
-  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(lane_top));
-  const float t = __uint_as_float(top);
-  scale = __fmul_rn(t, 1.0f / kMaxCode);
-  inv = rcp_fast(scale);
-  if (t < 0x1p-100f) scale = inv = 0.0f;
-  if (top >= 0x7F800000u) scale = inv = __uint_as_float(0x7FC00000u);
+// -sqrt(v), rounded to nearest, of nv = -v: with y = 1/sqrt(v) nearly, t = -v y
+// is nearly -sqrt(v), t^2 - v its exact residual (one fused operation), and
+// (t^2 - v) y / 2 what it is off by (Newton's step for t^2 = v; Markstein's
+// argument for why its rounding is the right one).  Equal to the correctly
+// rounded root for every float of the exponents from 2^-97 to 2^103; below 2^-100
+// the residual loses bits, and v below 2^-126 counts as (nearly) 0.
+__device__ __forceinline__ Two neg_sqrt(Two nv) {
+  const float2 x = apart(nv);
+  const Two y = two(rsqrt_fast(fmaxf(fabsf(x.x), 0x1p-126f)), rsqrt_fast(fmaxf(fabsf(x.y), 0x1p-126f)));
+  const Two t = nv * y;
+  return fma2(fma2(t, t, nv), y * both(0.5f), t);
 }
 
-// The code of a value r >= 0, given z = 2^-120 (r / scale): e4m3's grid is that
-// of z's bits above the lowest 20, its small evenly spaced values lying where
-// float's are.  The low bits and the random ones carry into the last kept bit
-// with the probability of z's distance from the lower neighbour.  What is not 0
-// becomes code 1 at least, and the largest code is 0x7E.
-__device__ __forceinline__ uint32_t round_stochastic(float z, float r, uint32_t bits16) {
-  const uint32_t w = max(__float_as_uint(z), min(__float_as_uint(r), 1u << 20));
-  return min(w + bits16 * 16u + 8u, 0x7EFFFFFu) >> 20;
+// Scales of a block's two moments, from each lane's largest magnitudes, and the
+// factors 448 / (largest), rounded to nearest, that take values to codes.
+// Below 2^-100 a block is zero; a value that is not finite makes it NaN.
+__device__ __forceinline__ void scales_of(float m_lane, float r_lane, float2& scale, float2& inv) {
+  // Magnitudes order as their bits do, NaN above infinity.
+  const float2 top = make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m_lane))),
+                                 __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r_lane))));
+  // The quotient by a reciprocal and its residual, as for the root; all times 2^-20, for the reciprocal of a large one.
+  const Two t = two(fmaxf(top.x, 0x1p-100f), fmaxf(top.y, 0x1p-100f)) * both(0x1p-20f);
+  const Two k = both(-kMaxCode * 0x1p-20f);
+  const float2 tt = apart(t);
+  const Two y = two(rcp_fast(-tt.x), rcp_fast(-tt.y));
+  const Two q = k * y;
+  inv = apart(fma2(fma2(q, t, k), y, q));
+  // top - top: 0, or NaN for what is not finite
+  scale = make_float2(__fmaf_rn(top.x, 1.0f / kMaxCode, __fsub_rn(top.x, top.x)),
+                      __fmaf_rn(top.y, 1.0f / kMaxCode, __fsub_rn(top.y, top.y)));
+  if (top.x < 0x1p-100f) scale.x = inv.x = 0.0f;
+  if (top.y < 0x1p-100f) scale.y = inv.y = 0.0f;
+}
+
+// The code of a value, given its negative (or +0) and z = 2^-120 (value / scale):
+// e4m3's grid is that of z's bits above the lowest 20, its small evenly spaced
+// values lying where float's are.  The low bits and the random ones carry into
+// the last kept bit with the probability of z's distance from the lower
+// neighbour.  What is not 0 becomes code 1 at least; the largest, within two of
+// z's last units of 448's, cannot be carried above 0x7E by less than 2^20 - 7.
+__device__ __forceinline__ uint32_t round_stochastic(float z, float neg, uint32_t bits16) {
+  // Signed: a z of -0 counts as less than 0.
+  const uint32_t w = (uint32_t)max(__float_as_int(z), (int)min(__float_as_uint(neg), 1u << 20));
+  return (w + bits16 * 16u + 8u) >> 20;
 }
 
 constexpr uint32_t kGolden = 0x9E3779B9u;
 
-template <typename P, typename G, bool MASTER>
+// One thread's elements of a chunk as they lie in memory.  W: the type of the
+// weights that are read, the master's where there are some.
+template <typename W, typename G>
+struct Fetched {
+  Words<W> w;
+  Words<G> g;
+  uint2 m, r;
+  float m_scale, r_scale;
+};
+
+template <typename W, typename G>
+__device__ __forceinline__ void fetch(const AdamEntry& e, const void* weights, int64_t at, Fetched<W, G>& x) {
+  x.w = load_words((const W*)weights + at);
+  x.g = load_words((const G*)e.grad + at);
+  x.m = *reinterpret_cast<const uint2*>((const uint8_t*)e.m + at);
+  x.r = *reinterpret_cast<const uint2*>((const uint8_t*)e.v + at);
+  x.m_scale = e.m_scale[at / kStateBlock];
+  x.r_scale = e.v_scale[at / kStateBlock];
+}
+
+// One thread's elements at `at`, fetched before where WHOLE.  All lanes of a
+// warp come here with the same WHOLE.
+template <bool WHOLE, typename P, typename G, bool MASTER, typename F>
 __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
-                                        float coef, int64_t at) {
+                                        float coef, int64_t at, const F& in) {
   const int64_t left = e.n - at;
   const int lane = threadIdx.x & 31;
-  if (left + lane * kOptVec <= 0) return;  // nothing of this block of states is in the tensor: the whole warp leaves
-  const int valid = (int)max((int64_t)0, min((int64_t)kOptVec, left));
+  if (!WHOLE && left + lane * kOptVec <= 0) return;  // no lane of the warp has elements
+  const int valid = WHOLE ? kOptVec : (int)max((int64_t)0, min((int64_t)kOptVec, left));
   const int64_t block = at / kStateBlock;
   P* p = (P*)e.param + at;
-  const G* g = (const G*)e.grad + at;
   float* w = e.master + at;
   uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
-  const bool whole = e.aligned && valid == kOptVec;
   float xp[kOptVec], xg[kOptVec], xm[kOptVec], xr[kOptVec];
   uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
-  if (whole) {
-    cm = *reinterpret_cast<const uint2*>(m);
-    cr = *reinterpret_cast<const uint2*>(v);
+  float m_scale, r_scale;
+  if (WHOLE) {
+    widen_words(in.w, xp);
+    widen_words(in.g, xg);
+    cm = in.m;
+    cr = in.r;
+    m_scale = in.m_scale;
+    r_scale = in.r_scale;
   } else {
+    if (MASTER) load_some(w, valid, xp);
+    else load_some(p, valid, xp);
+    load_some((const G*)e.grad + at, valid, xg);
 #pragma unroll
     for (int i = 0; i < kOptVec; ++i) {
       if (i < valid) {
@@ -267,44 +322,45 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
         (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
       }
     }
+    m_scale = e.m_scale[block];
+    r_scale = e.v_scale[block];
   }
-  if (MASTER) load_n(w, whole, valid, xp);
-  else load_n(p, whole, valid, xp);
-  load_n(g, whole, valid, xg);
-  const Two sm = both(__fmul_rn(e.m_scale[block], b.b1)), sr = both(__fmul_rn(e.v_scale[block], b.root_b2));
   codes_to_float(cm, xm);
   codes_to_float(cr, xr);
-  const Two kc = both(coef), km = both(b.one_m_b1), kr = both(b.root_one_m_b2), ki = both(f.inv_sqrt), ke = both(eps),
-            ks = both(-f.step), kd = both(f.decay);
+  const Two sm = both(m_scale), sr = both(r_scale), kc = both(coef);
+  const Two kb1 = both(b.b1), kg1 = both(b.one_m_b1), nb2 = both(-b.b2), ng2 = both(-b.one_m_b2);
+  const Two ki = both(-f.inv_sqrt), ke = both(eps), ks = both(-f.step), kd = both(f.decay);
   float m_top = 0.0f, r_top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kOptVec; i += 2) {
     const Two gi = two(xg[i], xg[i + 1]) * kc;
-    const Two mi = fma2(two(xm[i], xm[i + 1]), sm, gi * km);
-    // v = (sqrt(b2) r)^2 + (sqrt(1 - b2) g)^2
-    const Two a = two(xr[i], xr[i + 1]) * sr, c = gi * kr;
-    const float2 v2 = apart(fma2(a, a, c * c));
-    const float2 r2 = make_float2(sqrt_fast(v2.x), sqrt_fast(v2.y));
-    const float2 d = apart(fma2(two(r2.x, r2.y), ki, ke));
+    const Two mi = two(xm[i], xm[i + 1]) * sm * kb1 + gi * kg1;
+    const Two r = two(xr[i], xr[i + 1]) * sr;
+    const Two nr = neg_sqrt(r * r * nb2 + gi * gi * ng2);  // -v, and -sqrt(v) from here on
+    const float2 d = apart(fma2(nr, ki, ke));
     const float2 np = apart(fma2(mi * ks, two(rcp_fast(d.x), rcp_fast(d.y)), two(xp[i], xp[i + 1]) * kd));
-    const float2 nm = apart(mi);
+    const float2 m2 = apart(mi), r2 = apart(nr);
     xp[i] = np.x;
     xp[i + 1] = np.y;
     // Behind the tensor's end there is nothing: a block of NaN must not reach its scale from there.
-    xm[i] = i < valid ? nm.x : 0.0f;
-    xm[i + 1] = i + 1 < valid ? nm.y : 0.0f;
-    xr[i] = i < valid ? r2.x : 0.0f;
-    xr[i + 1] = i + 1 < valid ? r2.y : 0.0f;
-    m_top = max_nan(max_nan(m_top, fabsf(xm[i])), fabsf(xm[i + 1]));
-    r_top = max_nan(max_nan(r_top, xr[i]), xr[i + 1]);
+    xm[i] = WHOLE || i < valid ? m2.x : 0.0f;
+    xm[i + 1] = WHOLE || i + 1 < valid ? m2.y : 0.0f;
+    xr[i] = WHOLE || i < valid ? r2.x : 0.0f;
+    xr[i + 1] = WHOLE || i + 1 < valid ? r2.y : 0.0f;
+    m_top = max_nan(m_top, fabsf(xm[i]), fabsf(xm[i + 1]));
+    r_top = max_nan(r_top, fabsf(xr[i]), fabsf(xr[i + 1]));
   }
-  if (MASTER) store_n(w, whole, valid, xp);
-  store_n(p, whole, valid, xp);
-  float m_scale, m_inv, r_scale, r_inv;
-  scale_of(m_top, m_scale, m_inv);
-  scale_of(r_top, r_scale, r_inv);
+  if (WHOLE) {
+    if (MASTER) store_vec(w, xp);
+    store_vec(p, xp);
+  } else {
+    if (MASTER) store_some(w, valid, xp);
+    store_some(p, valid, xp);
+  }
+  float2 scale, inv;
+  scales_of(m_top, r_top, scale, inv);
   const uint32_t key = mix(f.key + (uint32_t)block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
-  const Two im = both(m_inv), ir = both(r_inv), grid = both(0x1p-120f);
+  const Two im = both(inv.x), ir = both(-inv.y), grid = both(0x1p-120f);
   uint32_t code[kOptVec];
 #pragma unroll
   for (int i = 0; i < kOptVec; i += 2) {
@@ -319,7 +375,7 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   cm = float_to_codes(xm);
   cr = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
                   code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
-  if (whole) {
+  if (WHOLE) {
     *reinterpret_cast<uint2*>(m) = cm;
     *reinterpret_cast<uint2*>(v) = cr;
   } else {
@@ -332,16 +388,18 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
     }
   }
   if (lane == 0) {
-    e.m_scale[block] = m_scale;
-    e.v_scale[block] = r_scale;
+    e.m_scale[block] = scale.x;
+    e.v_scale[block] = scale.y;
   }
 }
 
-template <typename P, typename G, bool MASTER, int BITS, int CAP>
-__global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ AdamTable<CAP> tab) {
-  __shared__ AdamFactors s_factors;
+// What every block of a step begins with: each tensor's factors into shared
+// memory, the clipping factor.  False where the step is to change nothing.
+template <int CAP>
+__device__ __forceinline__ bool begin_step(const AdamTable<CAP>& tab, AdamFactors* factors, float& coef) {
   const AdamHyper& h = tab.h;
-  float coef = 1.0f;
+  for (int i = threadIdx.x; i < tab.count; i += kOptThreads) factors[i] = factors_of(tab.t[i], h);
+  coef = 1.0f;
   bool take = true;
   if (h.part) {
     const double norm = norm_of(h.part, h.parts);
@@ -349,27 +407,16 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
     coef = clip_factor(norm, h.max_norm);
     take = isfinite(norm);  // the same in every block
   }
-  if (!take) return;
-  const Betas b = h.betas;
-  int i = tensor_of(tab.t, tab.count, blockIdx.x), last = -1;
-  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    while (c >= tab.t[i].end_chunk) ++i;
-    const AdamEntry& e = tab.t[i];
-    if (i != last) {
-      __syncthreads();
-      if (threadIdx.x == 0) s_factors = factors_of(e, h);
-      __syncthreads();
-      last = i;
-    }
-    const AdamFactors f = s_factors;
-    const int64_t at = (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
-    if (BITS == 32) update32<P, G, MASTER>(e, f, b, h.eps, coef, at);
-    else update8<P, G, MASTER>(e, f, b, h.eps, coef, at);
-  }
-  // The last block to come here has every other block's reads of the clocks
-  // behind it: it advances them, and leaves the ticket as it found it.
-  __shared__ bool s_last;
   __syncthreads();
+  return take;
+}
+
+// The last block to come here has every other block's reads of the clocks
+// behind it: it advances them, and leaves the ticket as it found it.
+template <int CAP>
+__device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
+  const AdamHyper& h = tab.h;
+  __shared__ bool s_last;
   if (threadIdx.x == 0) {
     __threadfence();
     s_last = atomicAdd(h.ticket, 1u) == gridDim.x - 1;
@@ -384,6 +431,61 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
     k[2] *= h.beta2;
   }
   if (threadIdx.x == 0) *h.ticket = 0;
+}
+
+__device__ __forceinline__ int64_t element_of(const AdamEntry& e, unsigned c) {
+  return (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
+}
+
+template <typename P, typename G, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ AdamTable<CAP> tab) {
+  __shared__ AdamFactors s_factors[CAP];
+  float coef;
+  if (!begin_step(tab, s_factors, coef)) return;
+  int i = tensor_of(tab.t, tab.count, blockIdx.x);
+  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    while (c >= tab.t[i].end_chunk) ++i;
+    const AdamEntry& e = tab.t[i];
+    update32<P, G, MASTER>(e, s_factors[i], tab.h.betas, tab.h.eps, coef, element_of(e, c));
+  }
+  end_step(tab);
+}
+
+// The arithmetic takes about as long as the memory: a thread's next elements
+// are on their way while it computes.
+template <typename P, typename G, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
+  using W = typename std::conditional<MASTER, float, P>::type;
+  __shared__ AdamFactors s_factors[CAP];
+  const auto whole_at = [&](const AdamEntry& e, int64_t at) { return e.aligned && (at | (kStateBlock - 1)) < e.n; };
+  const auto weights = [&](const AdamEntry& e) { return MASTER ? (const void*)e.master : e.param; };
+  int i = tensor_of(tab.t, tab.count, blockIdx.x);
+  int64_t at = element_of(tab.t[i], blockIdx.x);
+  bool whole = whole_at(tab.t[i], at);
+  Fetched<W, G> here, next;
+  if (whole) fetch(tab.t[i], weights(tab.t[i]), at, here);
+  float coef;
+  if (!begin_step(tab, s_factors, coef)) return;
+  for (unsigned c = blockIdx.x;;) {
+    const int this_i = i;
+    const int64_t this_at = at;
+    const bool this_whole = whole;
+    c += gridDim.x;
+    if (c < tab.chunks) {
+      while (c >= tab.t[i].end_chunk) ++i;
+      at = element_of(tab.t[i], c);
+      whole = whole_at(tab.t[i], at);
+      if (whole) fetch(tab.t[i], weights(tab.t[i]), at, next);
+    }
+    const AdamEntry& e = tab.t[this_i];
+    if (this_whole)
+      update8<true, P, G, MASTER>(e, s_factors[this_i], tab.h.betas, tab.h.eps, coef, this_at, here);
+    else
+      update8<false, P, G, MASTER>(e, s_factors[this_i], tab.h.betas, tab.h.eps, coef, this_at, here);
+    if (c >= tab.chunks) break;
+    here = next;
+  }
+  end_step(tab);
 }
 
 // One launch for the tensors of one combination of types, CAP at a time.
@@ -407,9 +509,18 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     }
     if (tab.count == 0) break;
     tab.chunks = (unsigned)chunks;
-    const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 8);
     DR_TB(ctx);
-    k_adamw<P, G, MASTER, BITS, CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+    if (BITS == 32) {
+      const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 8);
+      k_adamw<P, G, MASTER, CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+    } else {
+      auto* kernel = k_adamw8<P, G, MASTER, CAP>;
+      // One wave of blocks that stay.
+      int resident = 0;
+      DR_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kOptThreads, 0), "adamw8");
+      const unsigned blocks = std::min(tab.chunks, (unsigned)(ctx->num_sms * std::max(resident, 1)));
+      kernel<<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+    }
     DR_LAUNCHED(ctx, BITS == 32 ? "adamw" : "adamw8");
   }
   return DR_OK;
@@ -469,8 +580,7 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
                "adamw: tensor %d: lr_ratio and weight_decay must be finite and not negative", i);
   }
   AdamHyper h = {lr, beta1, beta2, max_norm, lr_device, (float)eps, nullptr, 0, norm, ticket,
-                 {(float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)std::sqrt(beta2),
-                  (float)std::sqrt(1.0 - beta2)}};
+                 {(float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2)}};
   if (max_norm > 0.0) {
     dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
     if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);

@@ -35,27 +35,41 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return
 template <>
 __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
 
-// kOptVec consecutive elements at a 16-byte aligned address.
+// kOptVec consecutive elements as they lie in memory, at a 16-byte aligned address.
 template <typename T>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[kOptVec]) {
-  constexpr int kWords = kOptVec * sizeof(T) / 16;
-  uint4 w[kWords];
+struct Words {
+  static constexpr int kCount = kOptVec * sizeof(T) / 16;
+  uint4 w[kCount];
+};
+
+template <typename T>
+__device__ __forceinline__ Words<T> load_words(const T* p) {
+  Words<T> x;
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-  const T* e = reinterpret_cast<const T*>(w);
+  for (int i = 0; i < Words<T>::kCount; ++i) x.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen_words(const Words<T>& words, float (&x)[kOptVec]) {
+  const T* e = reinterpret_cast<const T*>(words.w);
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) x[i] = widen(e[i]);
 }
 
 template <typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[kOptVec]) {
+  widen_words(load_words(p), x);
+}
+
+template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[kOptVec]) {
-  constexpr int kWords = kOptVec * sizeof(T) / 16;
-  uint4 w[kWords];
-  T* e = reinterpret_cast<T*>(w);
+  Words<T> words;
+  T* e = reinterpret_cast<T*>(words.w);
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) e[i] = narrow<T>(x[i]);
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  for (int i = 0; i < Words<T>::kCount; ++i) reinterpret_cast<uint4*>(p)[i] = words.w[i];
 }
 
 // `valid` (0 .. kOptVec) elements at any address of T's alignment; the others are 0.
