@@ -33,9 +33,9 @@ struct AdamEntry {
   int aligned;  // whether every vector of the tensor may be accessed whole
 };
 
-// beta1, beta2 and what they leave of 1.
+// beta1, beta2, what they leave of 1, and 1.
 struct Betas {
-  float b1, b2, one_m_b1, one_m_b2;
+  float b1, b2, one_m_b1, one_m_b2, one;
 };
 
 struct AdamHyper {
@@ -198,11 +198,6 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-  Two r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 // The hardware's approximations, within one or two units in the last place.
 __device__ __forceinline__ float rsqrt_fast(float x) {
   float r;
@@ -263,7 +258,7 @@ __device__ __forceinline__ void scales_of(float m_lane, float r_lane, float2& sc
 __device__ __forceinline__ uint32_t round_stochastic(float z, float neg, uint32_t bits16) {
   // Signed: a z of -0 counts as less than 0.
   const uint32_t w = (uint32_t)max(__float_as_int(z), (int)min(__float_as_uint(neg), 1u << 20));
-  return (w + bits16 * 16u + 8u) >> 20;
+  return (w + (bits16 << 4) + 8u) >> 20;
 }
 
 constexpr uint32_t kGolden = 0x9E3779B9u;
@@ -329,14 +324,17 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   codes_to_float(cr, xr);
   const Two sm = both(m_scale), sr = both(r_scale), kc = both(coef);
   const Two kb1 = both(b.b1), kg1 = both(b.one_m_b1), nb2 = both(-b.b2), ng2 = both(-b.one_m_b2);
+  // A sum of two products is a fused operation with a 1 that the compiler does
+  // not know: it would make a packed product and sum one, with one rounding.
+  const Two one = both(b.one);
   const Two ki = both(-f.inv_sqrt), ke = both(eps), ks = both(-f.step), kd = both(f.decay);
   float m_top = 0.0f, r_top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kOptVec; i += 2) {
     const Two gi = two(xg[i], xg[i + 1]) * kc;
-    const Two mi = two(xm[i], xm[i + 1]) * sm * kb1 + gi * kg1;
+    const Two mi = fma2(two(xm[i], xm[i + 1]) * sm * kb1, one, gi * kg1);
     const Two r = two(xr[i], xr[i + 1]) * sr;
-    const Two nr = neg_sqrt(r * r * nb2 + gi * gi * ng2);  // -v, and -sqrt(v) from here on
+    const Two nr = neg_sqrt(fma2(r * r * nb2, one, gi * gi * ng2));  // -v, and -sqrt(v) from here on
     const float2 d = apart(fma2(nr, ki, ke));
     const float2 np = apart(fma2(mi * ks, two(rcp_fast(d.x), rcp_fast(d.y)), two(xp[i], xp[i + 1]) * kd));
     const float2 m2 = apart(mi), r2 = apart(nr);
@@ -580,7 +578,7 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
                "adamw: tensor %d: lr_ratio and weight_decay must be finite and not negative", i);
   }
   AdamHyper h = {lr, beta1, beta2, max_norm, lr_device, (float)eps, nullptr, 0, norm, ticket,
-                 {(float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2)}};
+                 {(float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), 1.0f}};
   if (max_norm > 0.0) {
     dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
     if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);
