@@ -60,6 +60,7 @@ BLOCK = 256  # elements that share the scale of an 8-bit state
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # dr_dtype
 _DTYPE = operator.attrgetter("dtype")
 _SHAPE = operator.attrgetter("shape")
+_LAYOUT = operator.attrgetter("layout")
 _T = torch.Tensor
 
 # dr_grad_tensor and dr_adamw_tensor
@@ -86,6 +87,10 @@ def _check_list(tensors, what: str):
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not ts:
         raise ValueError(f"{what}: no tensors")
+    if (all(isinstance(t, torch.Tensor) for t in ts) and set(map(_LAYOUT, ts)) == {torch.strided} and
+            len(places := set(map(_T.get_device, ts))) == 1 and min(places) >= 0 and
+            _TYPES.keys() >= set(map(_DTYPE, ts))):
+        return ts
     for t in ts:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: torch.Tensor expected (got {type(t).__name__})")
@@ -102,24 +107,51 @@ def _check_list(tensors, what: str):
 
 def _check_apart(ts, what: str):
     """Refuses a list in which two tensors share memory: an element would be updated twice."""
-    spans = np.array([(t.data_ptr(), t.numel() * t.element_size()) for t in ts if t.numel()], np.uint64).reshape(-1, 2)
-    spans = spans[np.argsort(spans[:, 0])]
-    if (spans[:-1, 0] + spans[:-1, 1] > spans[1:, 0]).any():
+    begin = np.array(list(map(_T.data_ptr, ts)), np.uint64)
+    size = np.array(list(map(_T.nelement, ts)), np.uint64) * np.array(list(map(_T.element_size, ts)), np.uint64)
+    some = size > 0
+    if not some.all():
+        begin, size = begin[some], size[some]
+    order = np.argsort(begin)
+    begin, size = begin[order], size[order]
+    if (begin[:-1] + size[:-1] > begin[1:]).any():
         raise ValueError(f"{what}: two of the tensors share memory")
 
 
 def _grad_table(ts):
     tab = np.zeros(len(ts), _GRAD_ROW)
     tab["data"] = list(map(_T.data_ptr, ts))
-    tab["n"] = list(map(_T.numel, ts))
-    tab["type"] = [_TYPES[d] for d in map(_DTYPE, ts)]
+    tab["n"] = list(map(_T.nelement, ts))
+    tab["type"] = list(map(_TYPES.__getitem__, map(_DTYPE, ts)))
     return tab
 
 
+def _context(index: int):
+    """The context of a device, on torch's current stream there."""
+    c = L.ctx_for(index)
+    L.lib().dr_ctx_set_stream(c, torch._C._cuda_getCurrentRawStream(index))
+    return c
+
+
 def _norm_work(c, count: int, dev) -> torch.Tensor:
-    # From torch's allocator at each call: it belongs to the stream (or to the
-    # graph being captured) and to no other call.
     return torch.empty(int(L.lib().dr_grad_norm_work_bytes(c, count)) // 8, dtype=torch.float64, device=dev)
+
+
+def _norm_call(fn, ts, what: str, *args) -> torch.Tensor:
+    """fn (dr_grad_norm or dr_clip_grad_norm) on the list; the norm."""
+    index = ts[0].get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _norm_call(fn, ts, what, *args)
+    c = _context(index)
+    dev = ts[0].device
+    # From torch's allocator at each call: both belong to the stream (or to the
+    # graph being captured) and to no other call.
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    work = _norm_work(c, len(ts), dev)
+    tab = _grad_table(ts)
+    L.check(fn(c, tab.ctypes.data, len(ts), *args, norm.data_ptr(), work.data_ptr()), c, what)
+    return norm
 
 
 def grad_norm(grads) -> torch.Tensor:
@@ -127,16 +159,10 @@ def grad_norm(grads) -> torch.Tensor:
     tensors, in any mix of float32, bfloat16 and float16): a float32 scalar on
     their device, the same from run to run.  Squares are summed in 64 bits, so
     the norm is finite wherever float32 holds it."""
-    ts = [t.detach() for t in _check_list(grads, "grad_norm")]
-    ts = [t if _dense(t) else t.contiguous() for t in ts]
-    dev = ts[0].device
-    with torch.cuda.device(dev):
-        c = _ctx(ts[0])
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        work = _norm_work(c, len(ts), dev)
-        tab = _grad_table(ts)
-        L.check(L.lib().dr_grad_norm(c, tab.ctypes.data, len(ts), _ptr(norm), _ptr(work)), c, "grad_norm")
-    return norm
+    ts = _check_list(grads, "grad_norm")
+    if not all(map(_T.is_contiguous, ts)):
+        ts = [t if _dense(t) else t.detach().contiguous() for t in ts]
+    return _norm_call(L.lib().dr_grad_norm, ts, "grad_norm")
 
 
 def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
@@ -146,20 +172,12 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
     formula does."""
     ts = _check_list(grads, "clip_grad_norm_")
     max_norm = float(max_norm)
-    if not (max_norm > 0.0 and math.isfinite(max_norm)):
+    if not 0.0 < max_norm < 1e300:
         raise ValueError(f"clip_grad_norm_: max_norm must be positive and finite (got {max_norm})")
-    for t in ts:
-        if not _dense(t):
-            raise ValueError("clip_grad_norm_: tensors must fill their memory (they are scaled in place)")
+    if not all(map(_T.is_contiguous, ts)) and not all(map(_dense, ts)):
+        raise ValueError("clip_grad_norm_: tensors must fill their memory (they are scaled in place)")
     _check_apart(ts, "clip_grad_norm_")
-    dev = ts[0].device
-    with torch.cuda.device(dev):
-        c = _ctx(ts[0])
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        work = _norm_work(c, len(ts), dev)
-        tab = _grad_table(ts)
-        L.check(L.lib().dr_clip_grad_norm(c, tab.ctypes.data, len(ts), max_norm, _ptr(norm), _ptr(work)), c,
-                "clip_grad_norm_")
+    norm = _norm_call(L.lib().dr_clip_grad_norm, ts, "clip_grad_norm_", max_norm)
     torch.autograd.graph.increment_version(ts)
     return norm
 
@@ -266,12 +284,23 @@ class AdamW:
         tab["seed"] = (self.seed + np.arange(count, dtype=np.uint64).astype(object) * 0x9E3779B9) % (1 << 32)
         tab["param_type"] = [_TYPES[p.dtype] for p in self.params]
         self._tab = tab
+        # A step updates the memory that it was given: these keep it alive, and
+        # the parameters must still be there.
+        self._held = [p.detach() for p in self.params]
+        self._addresses = tab["param"][:] = list(map(_T.data_ptr, self.params))
+        self._col_grad, self._col_type, self._at = tab["grad"], tab["grad_type"], tab.ctypes.data
+        self._index, self._device = dev.index, dev
+        with torch.cuda.device(dev):
+            # A step's own: steps of one optimizer never run side by side.
+            self._work = _norm_work(_context(dev.index), count, dev)
+        self._ticket_at, self._work_at = self._ticket.data_ptr(), self._work.data_ptr()
         # What a step's gradients are held against.
         self._shapes = list(map(_SHAPE, self.params))
         self._strides = list(map(_T.stride, self.params))
         self._dtypes = list(map(_DTYPE, self.params))
-        self._places = list(map(_T.get_device, self.params))
+        self._places = [dev.index] * count
         self._plain = all(map(_T.is_contiguous, self.params))
+        self._seen = None  # the gradients' types that _col_type says
 
     @staticmethod
     def _memory_order(t: torch.Tensor) -> torch.Tensor:
@@ -325,41 +354,48 @@ class AdamW:
         it is; default: the parameters' .grad).  Gradients have their parameter's
         shape and type, or one of the two is float32.  Returns the norm of the
         gradients (a float32 scalar on the device) with max_grad_norm, else None."""
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.step(grads)
         ps = self.params
         gs = [p.grad for p in ps] if grads is None else list(grads)
         if len(gs) != len(ps):
             raise ValueError(f"AdamW: {len(ps)} gradients expected (got {len(gs)})")
         lr, lr_dev, top = self._step_args()
-        if lr_dev is not None and lr_dev.device != ps[0].device:
+        if lr_dev is not None and lr_dev.get_device() != self._index:
             raise ValueError("AdamW: a learning_rate tensor must be on the parameters' device")
-        if (list(map(_SHAPE, ps)) != self._shapes or list(map(_DTYPE, ps)) != self._dtypes or
-                list(map(_T.stride, ps)) != self._strides or list(map(_T.get_device, ps)) != self._places):
-            raise ValueError("AdamW: a parameter has another shape, layout, type or device than when it was given")
-        dev = ps[0].device
-        with torch.cuda.device(dev):
-            try:
-                fast = (self._plain and list(map(_SHAPE, gs)) == self._shapes and
-                        list(map(_DTYPE, gs)) == self._dtypes and list(map(_T.get_device, gs)) == self._places and
-                        all(map(_T.is_contiguous, gs)))
-            except (AttributeError, TypeError):
-                fast = False  # a None among them, or not a tensor
-            if not fast:
+        if list(map(_T.data_ptr, ps)) != self._addresses:
+            raise ValueError("AdamW: a parameter is at another address than when it was given")
+        at, count, rows = ps, len(ps), None
+        try:
+            types = list(map(_DTYPE, gs))
+            if (types != self._seen or not self._plain or list(map(_SHAPE, gs)) != self._shapes or
+                    list(map(_T.get_device, gs)) != self._places or not all(map(_T.is_contiguous, gs))):
                 gs = self._gradients(gs)
-            tab, at = self._tab.copy(), ps
-            if not fast and any(g is None for g in gs):
-                keep = [i for i, g in enumerate(gs) if g is not None]
-                tab, at, gs = tab[keep], [ps[i] for i in keep], [gs[i] for i in keep]
-            tab["param"] = list(map(_T.data_ptr, at))
-            tab["grad"] = list(map(_T.data_ptr, gs))
-            tab["grad_type"] = tab["param_type"] if fast else [_TYPES[g.dtype] for g in gs]
-            c = _ctx(ps[0])
-            norm = work = None
-            if top:
-                norm = torch.empty((), dtype=torch.float32, device=dev)
-                work = _norm_work(c, len(gs), dev)
-            L.check(L.lib().dr_adamw_step(c, tab.ctypes.data, len(gs), lr, _ptr(lr_dev), self.beta1, self.beta2,
-                                          self.eps, self.state_bits, top, _ptr(norm), _ptr(work),
-                                          _ptr(self._ticket)), c, "AdamW")
+                types = None
+        except (AttributeError, TypeError):  # a None among them, or not a tensor
+            gs = self._gradients(gs)
+            types = None
+        if types is None:
+            keep = [i for i, g in enumerate(gs) if g is not None]
+            if len(keep) == count:
+                self._seen = list(map(_DTYPE, gs))
+                self._col_type[:] = [_TYPES[d] for d in self._seen]
+            else:
+                at, count, gs = [ps[i] for i in keep], len(keep), [gs[i] for i in keep]
+                rows = self._tab[keep]
+                rows["grad"] = list(map(_T.data_ptr, gs))
+                rows["grad_type"] = [_TYPES[g.dtype] for g in gs]
+        if rows is None:
+            self._col_grad[:] = list(map(_T.data_ptr, gs))
+        c = _context(self._index)
+        norm = torch.empty((), dtype=torch.float32, device=self._device) if top else None
+        status = L.lib().dr_adamw_step(
+            c, self._at if rows is None else rows.ctypes.data, count, lr, None if lr_dev is None else lr_dev.data_ptr(),
+            self.beta1, self.beta2, self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(),
+            self._work_at, self._ticket_at)
+        if status:
+            L.check(status, c, "AdamW")
         torch.autograd.graph.increment_version(at)
         return norm
 
