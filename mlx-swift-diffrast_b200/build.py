@@ -4,7 +4,8 @@
 
 Objects go to mlx-swift-diffrast_b200/_build/, the shared library to
 mlx-swift-diffrast_b200/diffrast/libdiffrast.so (in-tree, next to the Python
-binding that loads it).  A file is recompiled when it or any header changed.
+binding that loads it), the host-side Python extension of the optimizer to
+diffrast/_rows.so.  A file is recompiled when it or any header changed.
 """
 from __future__ import annotations
 
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -82,7 +84,26 @@ def build(force: bool = False, jobs: int = 0, verbose_ptxas: bool = False) -> st
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_rows(force)
     return LIB
+
+
+ROWS_SRC = os.path.join(PKG, "pyext", "rows.cpp")
+ROWS = os.path.join(PKG, "diffrast", "_rows.so")
+
+
+def build_rows(force: bool = False) -> str:
+    """The Python extension of the optimizer's host path (pyext/rows.cpp): host
+    compiler only, linked against nothing."""
+    if not force and os.path.exists(ROWS) and os.path.getmtime(ROWS) >= max(
+            os.path.getmtime(ROWS_SRC), os.path.getmtime(__file__), *[os.path.getmtime(h) for h in _headers()]):
+        return ROWS
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"], ROWS_SRC, "-o", ROWS]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"extension build failed:\n{r.stdout}\n{r.stderr}")
+    return ROWS
 
 
 DRIVER_SRC = os.path.join(PKG, "cdriver", "dr_check.cpp")

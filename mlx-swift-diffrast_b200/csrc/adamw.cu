@@ -498,11 +498,11 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
       const dr_adamw_tensor& x = t[i];
       if (x.n == 0 || x.param_type != pt || x.grad_type != gt || (x.master != nullptr) != MASTER) continue;
       const uintptr_t state = (uintptr_t)x.m | (uintptr_t)x.v;
-      const int aligned = (((uintptr_t)x.param | (uintptr_t)x.grad | (uintptr_t)x.master) & 15) == 0 &&
-                          (state & (BITS == 32 ? 15 : 7)) == 0;
-      tab.t[tab.count++] = {x.param,   x.grad, x.master, x.m,        x.v,            x.m_scale, x.v_scale,
-                            x.clock,   x.n,    x.lr_ratio, x.weight_decay, x.seed, (unsigned)chunks, (unsigned)(chunks + opt_chunks(x.n)),
-                            aligned};
+      const uintptr_t vectors = (uintptr_t)x.param | (uintptr_t)x.grad | (uintptr_t)x.master;
+      const int aligned = ((vectors & 15) | (state & (BITS == 32 ? 15 : 7))) == 0;
+      tab.t[tab.count++] = {x.param,   x.grad,     x.master,       x.m,    x.v,
+                            x.m_scale, x.v_scale,  x.clock,        x.n,    x.lr_ratio,
+                            x.weight_decay, x.seed, (unsigned)chunks, (unsigned)(chunks + opt_chunks(x.n)), aligned};
       chunks += opt_chunks(x.n);
     }
     if (tab.count == 0) break;

@@ -8,13 +8,13 @@ in fp32, bf16 or fp16, AdamW's states in 32 or in 8 bits.
 from __future__ import annotations
 
 import math
-import operator
 from typing import Optional, Sequence, Union
 
 import numpy as np
 import torch
 
 from . import _lib as L
+from . import _rows
 from .ops import _ctx, _f32, _ptr
 
 
@@ -58,10 +58,7 @@ class Adam:
 BLOCK = 256  # elements that share the scale of an 8-bit state
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # dr_dtype
-_DTYPE = operator.attrgetter("dtype")
-_SHAPE = operator.attrgetter("shape")
-_LAYOUT = operator.attrgetter("layout")
-_T = torch.Tensor
+_CUDA = [torch.device("cuda", i) for i in range(64)]
 
 # dr_grad_tensor and dr_adamw_tensor
 _GRAD_ROW = np.dtype([("data", "u8"), ("n", "i8"), ("type", "i4"), ("reserved", "i4")])
@@ -87,10 +84,6 @@ def _check_list(tensors, what: str):
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not ts:
         raise ValueError(f"{what}: no tensors")
-    if (all(isinstance(t, torch.Tensor) for t in ts) and set(map(_LAYOUT, ts)) == {torch.strided} and
-            len(places := set(map(_T.get_device, ts))) == 1 and min(places) >= 0 and
-            _TYPES.keys() >= set(map(_DTYPE, ts))):
-        return ts
     for t in ts:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: torch.Tensor expected (got {type(t).__name__})")
@@ -107,11 +100,9 @@ def _check_list(tensors, what: str):
 
 def _check_apart(ts, what: str):
     """Refuses a list in which two tensors share memory: an element would be updated twice."""
-    begin = np.array(list(map(_T.data_ptr, ts)), np.uint64)
-    size = np.array(list(map(_T.nelement, ts)), np.uint64) * np.array(list(map(_T.element_size, ts)), np.uint64)
-    some = size > 0
-    if not some.all():
-        begin, size = begin[some], size[some]
+    begin = np.array([t.data_ptr() for t in ts], np.uint64)
+    size = np.array([t.numel() * t.element_size() for t in ts], np.uint64)
+    begin, size = begin[size > 0], size[size > 0]
     order = np.argsort(begin)
     begin, size = begin[order], size[order]
     if (begin[:-1] + size[:-1] > begin[1:]).any():
@@ -120,9 +111,9 @@ def _check_apart(ts, what: str):
 
 def _grad_table(ts):
     tab = np.zeros(len(ts), _GRAD_ROW)
-    tab["data"] = list(map(_T.data_ptr, ts))
-    tab["n"] = list(map(_T.nelement, ts))
-    tab["type"] = list(map(_TYPES.__getitem__, map(_DTYPE, ts)))
+    tab["data"] = [t.data_ptr() for t in ts]
+    tab["n"] = [t.numel() for t in ts]
+    tab["type"] = [_TYPES[t.dtype] for t in ts]
     return tab
 
 
@@ -137,20 +128,27 @@ def _norm_work(c, count: int, dev) -> torch.Tensor:
     return torch.empty(int(L.lib().dr_grad_norm_work_bytes(c, count)) // 8, dtype=torch.float64, device=dev)
 
 
-def _norm_call(fn, ts, what: str, *args) -> torch.Tensor:
-    """fn (dr_grad_norm or dr_clip_grad_norm) on the list; the norm."""
-    index = ts[0].get_device()
+def _norm_call(fn, ts, what: str, apart: bool, dense, *args) -> torch.Tensor:
+    """fn (dr_grad_norm or dr_clip_grad_norm) on the list `ts`; the norm.  dense: what the tensors become that are not
+    contiguous."""
+    found = _rows.grads(ts, apart)
+    if found is None:
+        ts = [t if t.is_contiguous() else dense(t) for t in _check_list(ts, what)]
+        if apart:
+            _check_apart(ts, what)
+        found = ts[0].get_device(), _grad_table(ts).tobytes()
+    index, rows = found
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            return _norm_call(fn, ts, what, *args)
+            return _norm_call(fn, ts, what, apart, dense, *args)
     c = _context(index)
-    dev = ts[0].device
     # From torch's allocator at each call: both belong to the stream (or to the
     # graph being captured) and to no other call.
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    work = _norm_work(c, len(ts), dev)
-    tab = _grad_table(ts)
-    L.check(fn(c, tab.ctypes.data, len(ts), *args, norm.data_ptr(), work.data_ptr()), c, what)
+    norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
+    work = _norm_work(c, len(ts), _CUDA[index])
+    status = fn(c, rows, len(ts), *args, norm.data_ptr(), work.data_ptr())
+    if status:
+        L.check(status, c, what)
     return norm
 
 
@@ -159,10 +157,9 @@ def grad_norm(grads) -> torch.Tensor:
     tensors, in any mix of float32, bfloat16 and float16): a float32 scalar on
     their device, the same from run to run.  Squares are summed in 64 bits, so
     the norm is finite wherever float32 holds it."""
-    ts = _check_list(grads, "grad_norm")
-    if not all(map(_T.is_contiguous, ts)):
-        ts = [t if _dense(t) else t.detach().contiguous() for t in ts]
-    return _norm_call(L.lib().dr_grad_norm, ts, "grad_norm")
+    ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    return _norm_call(L.lib().dr_grad_norm, ts, "grad_norm", False,
+                      lambda t: t if _dense(t) else t.detach().contiguous())
 
 
 def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
@@ -170,14 +167,17 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
     place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had.
     The factor stays on the device.  A NaN or infinite norm gives what the
     formula does."""
-    ts = _check_list(grads, "clip_grad_norm_")
+    ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     max_norm = float(max_norm)
-    if not 0.0 < max_norm < 1e300:
+    if ts and not 0.0 < max_norm < 1e300:
         raise ValueError(f"clip_grad_norm_: max_norm must be positive and finite (got {max_norm})")
-    if not all(map(_T.is_contiguous, ts)) and not all(map(_dense, ts)):
-        raise ValueError("clip_grad_norm_: tensors must fill their memory (they are scaled in place)")
-    _check_apart(ts, "clip_grad_norm_")
-    norm = _norm_call(L.lib().dr_clip_grad_norm, ts, "clip_grad_norm_", max_norm)
+
+    def dense(t):
+        if not _dense(t):
+            raise ValueError("clip_grad_norm_: tensors must fill their memory (they are scaled in place)")
+        return t
+
+    norm = _norm_call(L.lib().dr_clip_grad_norm, ts, "clip_grad_norm_", True, dense, max_norm)
     torch.autograd.graph.increment_version(ts)
     return norm
 
@@ -287,20 +287,17 @@ class AdamW:
         # A step updates the memory that it was given: these keep it alive, and
         # the parameters must still be there.
         self._held = [p.detach() for p in self.params]
-        self._addresses = tab["param"][:] = list(map(_T.data_ptr, self.params))
-        self._col_grad, self._col_type, self._at = tab["grad"], tab["grad_type"], tab.ctypes.data
+        self._addresses = tab["param"][:] = [p.data_ptr() for p in self.params]
+        self._at = tab.ctypes.data
         self._index, self._device = dev.index, dev
         with torch.cuda.device(dev):
             # A step's own: steps of one optimizer never run side by side.
             self._work = _norm_work(_context(dev.index), count, dev)
         self._ticket_at, self._work_at = self._ticket.data_ptr(), self._work.data_ptr()
         # What a step's gradients are held against.
-        self._shapes = list(map(_SHAPE, self.params))
-        self._strides = list(map(_T.stride, self.params))
-        self._dtypes = list(map(_DTYPE, self.params))
-        self._places = [dev.index] * count
-        self._plain = all(map(_T.is_contiguous, self.params))
-        self._seen = None  # the gradients' types that _col_type says
+        self._shapes = [p.shape for p in self.params]
+        self._strides = [p.stride() for p in self.params]
+        self._dtypes = [p.dtype for p in self.params]
 
     @staticmethod
     def _memory_order(t: torch.Tensor) -> torch.Tensor:
@@ -339,7 +336,7 @@ class AdamW:
             if g.shape != self._shapes[i]:
                 raise ValueError(f"AdamW: gradient {i} has shape {tuple(g.shape)}, its parameter "
                                  f"{tuple(self._shapes[i])}")
-            if g.get_device() != self._places[i]:
+            if g.get_device() != self._index:
                 raise ValueError(f"AdamW: gradient {i} is not on its parameter's device")
             p = self._dtypes[i]
             if g.dtype not in _TYPES or not (g.dtype == p or torch.float32 in (p, g.dtype)):
@@ -358,40 +355,26 @@ class AdamW:
             with torch.cuda.device(self._index):
                 return self.step(grads)
         ps = self.params
-        gs = [p.grad for p in ps] if grads is None else list(grads)
-        if len(gs) != len(ps):
-            raise ValueError(f"AdamW: {len(ps)} gradients expected (got {len(gs)})")
         lr, lr_dev, top = self._step_args()
         if lr_dev is not None and lr_dev.get_device() != self._index:
             raise ValueError("AdamW: a learning_rate tensor must be on the parameters' device")
-        if list(map(_T.data_ptr, ps)) != self._addresses:
-            raise ValueError("AdamW: a parameter is at another address than when it was given")
-        at, count, rows = ps, len(ps), None
-        try:
-            types = list(map(_DTYPE, gs))
-            if (types != self._seen or not self._plain or list(map(_SHAPE, gs)) != self._shapes or
-                    list(map(_T.get_device, gs)) != self._places or not all(map(_T.is_contiguous, gs))):
-                gs = self._gradients(gs)
-                types = None
-        except (AttributeError, TypeError):  # a None among them, or not a tensor
+        at, rows = ps, self._at
+        if _rows.step(ps, grads, self._tab, self._index) != 0:
+            gs = [p.grad for p in ps] if grads is None else list(grads)
+            if len(gs) != len(ps):
+                raise ValueError(f"AdamW: {len(ps)} gradients expected (got {len(gs)})")
+            if [p.data_ptr() for p in ps] != self._addresses:
+                raise ValueError("AdamW: a parameter is at another address than when it was given")
             gs = self._gradients(gs)
-            types = None
-        if types is None:
             keep = [i for i, g in enumerate(gs) if g is not None]
-            if len(keep) == count:
-                self._seen = list(map(_DTYPE, gs))
-                self._col_type[:] = [_TYPES[d] for d in self._seen]
-            else:
-                at, count, gs = [ps[i] for i in keep], len(keep), [gs[i] for i in keep]
-                rows = self._tab[keep]
-                rows["grad"] = list(map(_T.data_ptr, gs))
-                rows["grad_type"] = [_TYPES[g.dtype] for g in gs]
-        if rows is None:
-            self._col_grad[:] = list(map(_T.data_ptr, gs))
+            at, gs, table = [ps[i] for i in keep], [gs[i] for i in keep], self._tab[keep]
+            table["grad"] = [g.data_ptr() for g in gs]
+            table["grad_type"] = [_TYPES[g.dtype] for g in gs]
+            rows = table.tobytes()
         c = _context(self._index)
         norm = torch.empty((), dtype=torch.float32, device=self._device) if top else None
         status = L.lib().dr_adamw_step(
-            c, self._at if rows is None else rows.ctypes.data, count, lr, None if lr_dev is None else lr_dev.data_ptr(),
+            c, rows, len(at), lr, None if lr_dev is None else lr_dev.data_ptr(),
             self.beta1, self.beta2, self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(),
             self._work_at, self._ticket_at)
         if status:
