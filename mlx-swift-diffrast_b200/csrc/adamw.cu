@@ -28,8 +28,6 @@ struct AdamEntry {
   int64_t n;
   double lr_ratio, weight_decay;
   uint32_t seed;
-  unsigned first_chunk;
-  unsigned end_chunk;
   int aligned;  // whether every vector of the tensor may be accessed whole
 };
 
@@ -53,11 +51,12 @@ struct AdamHyper {
 template <int CAP>
 struct AdamTable {
   AdamEntry t[CAP];
+  unsigned first[CAP];  // each tensor's first chunk
   AdamHyper h;
   int count;
   unsigned chunks;
 };
-constexpr int kSmall = 32, kLarge = 304;
+constexpr int kSmall = 32, kLarge = 300;
 static_assert(sizeof(AdamTable<kSmall>) <= 4096 && sizeof(AdamTable<kLarge>) <= 32764, "kernel parameters");
 
 // What a step's elements share: for tensor e at its step t.
@@ -88,6 +87,49 @@ __device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const Adam
   return f;
 }
 
+// 8-bit states: a warp holds a block of 256 elements, eight to a lane.
+constexpr int kStateBlock = 256;
+static_assert(kStateBlock == 32 * kOptVec && kOptChunk % kStateBlock == 0, "one block of states to a warp");
+
+// A chunk: its tensor's factors, and where it begins.
+struct AdamSlot {
+  AdamFactors f;
+  const void* weights;  // that are read: the master's where there are some
+  void* param;
+  const void* grad;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  uint32_t block;  // of states, from the tensor's first on
+  int valid;       // elements
+  int aligned;
+};
+
+template <typename P, typename G, bool MASTER, int BITS, int CAP>
+__device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, AdamSlot& slot) {
+  if (c >= tab.chunks) return;
+  const int i = tensor_of(tab.first, tab.count, c);
+  const AdamEntry& e = tab.t[i];
+  const int64_t at = (int64_t)(c - tab.first[i]) * kOptChunk;
+  const AdamFactors f = factors_of(e, tab.h);
+  if (threadIdx.x % 32 != 0) return;
+  constexpr int kState = BITS == 32 ? 4 : 1;
+  slot.f = f;
+  slot.weights = MASTER ? (const void*)(e.master + at) : (const P*)e.param + at;
+  slot.param = (P*)e.param + at;
+  slot.grad = (const G*)e.grad + at;
+  slot.m = (char*)e.m + at * kState;
+  slot.v = (char*)e.v + at * kState;
+  slot.block = (uint32_t)(at / kStateBlock);
+  if (BITS == 8) {
+    slot.m_scale = e.m_scale + at / kStateBlock;
+    slot.v_scale = e.v_scale + at / kStateBlock;
+  }
+  slot.valid = (int)min((int64_t)kOptChunk, e.n - at);
+  slot.aligned = e.aligned;
+}
+
 __device__ __forceinline__ float next_m(const Betas& b, float m, float g) {
   return __fadd_rn(__fmul_rn(m, b.b1), __fmul_rn(g, b.one_m_b1));
 }
@@ -112,16 +154,15 @@ __device__ __forceinline__ void store_n(T* p, bool whole, int valid, const float
   else store_some(p, valid, x);
 }
 
-// 32-bit states: one thread's elements at `at`.
+// 32-bit states: one thread's elements of a chunk.
 template <typename P, typename G, bool MASTER>
-__device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
-                                         float coef, int64_t at) {
-  const int64_t left = e.n - at;
-  if (left <= 0) return;
-  const int valid = (int)min((int64_t)kOptVec, left);
+__device__ __forceinline__ void update32(const AdamSlot& e, const Betas& b, float eps, float coef) {
+  const unsigned at = threadIdx.x * kOptVec;
+  const int valid = min(kOptVec, e.valid - (int)at);
+  if (valid <= 0) return;
   P* p = (P*)e.param + at;
   const G* g = (const G*)e.grad + at;
-  float* w = e.master + at;
+  float* w = (float*)e.weights + at;
   float *m = (float*)e.m + at, *v = (float*)e.v + at;
   const bool whole = e.aligned && valid == kOptVec;
   float xp[kOptVec], xg[kOptVec], xm[kOptVec], xv[kOptVec];
@@ -130,6 +171,7 @@ __device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& 
   load_n(g, whole, valid, xg);
   load_n(m, whole, valid, xm);
   load_n(v, whole, valid, xv);
+  const AdamFactors f = e.f;
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) {
     const float gi = __fmul_rn(xg[i], coef);
@@ -143,9 +185,6 @@ __device__ __forceinline__ void update32(const AdamEntry& e, const AdamFactors& 
   store_n(p, whole, valid, xp);
 }
 
-// 8-bit states: a warp holds a block of 256 elements, eight to a lane.
-constexpr int kStateBlock = 256;
-static_assert(kStateBlock == 32 * kOptVec && kOptChunk % kStateBlock == 0, "one block of states to a warp");
 constexpr float kMaxCode = 448.0f;  // e4m3's largest
 
 __device__ __forceinline__ void codes_to_float(uint2 c, float (&x)[kOptVec]) {
@@ -251,14 +290,22 @@ __device__ __forceinline__ void scales_of(float m_lane, float r_lane, float2& sc
 
 // The code of a value, given its negative (or +0) and z = 2^-120 (value / scale):
 // e4m3's grid is that of z's bits above the lowest 20, its small evenly spaced
-// values lying where float's are.  The low bits and the random ones carry into
-// the last kept bit with the probability of z's distance from the lower
-// neighbour.  What is not 0 becomes code 1 at least; the largest, within two of
-// z's last units of 448's, cannot be carried above 0x7E by less than 2^20 - 7.
-__device__ __forceinline__ uint32_t round_stochastic(float z, float neg, uint32_t bits16) {
+// values lying where float's are.  The low bits and the random ones (16 of them
+// and half of their last one's worth) carry into the last kept bit with the
+// probability of z's distance from the lower neighbour.  What is not 0 becomes
+// code 1 at least; the largest, within two of z's last units of 448's, cannot be
+// carried above 0x7E by less than 2^20 - 7.  The code is in the highest byte,
+// the others are what is cut off.  HALF: which 16 bits of `word`.
+template <int HALF>
+__device__ __forceinline__ uint32_t round_stochastic(float z, float neg, uint32_t word) {
   // Signed: a z of -0 counts as less than 0.
   const uint32_t w = (uint32_t)max(__float_as_int(z), (int)min(__float_as_uint(neg), 1u << 20));
-  return (w + (bits16 << 4) + 8u) >> 20;
+  // 2^4 (16 bits16 + 8): bytes 0x80, bits16's low and high one, 0.
+  return (w << 4) + __byte_perm(word, 0x80u, HALF ? 0x5324 : 0x5104);
+}
+// The highest bytes of four words.
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
 constexpr uint32_t kGolden = 0x9E3779B9u;
@@ -274,27 +321,26 @@ struct Fetched {
 };
 
 template <typename W, typename G>
-__device__ __forceinline__ void fetch(const AdamEntry& e, const void* weights, int64_t at, Fetched<W, G>& x) {
-  x.w = load_words((const W*)weights + at);
+__device__ __forceinline__ void fetch(const AdamSlot& e, Fetched<W, G>& x) {
+  const unsigned at = threadIdx.x * kOptVec;
+  x.w = load_words((const W*)e.weights + at);
   x.g = load_words((const G*)e.grad + at);
   x.m = *reinterpret_cast<const uint2*>((const uint8_t*)e.m + at);
   x.r = *reinterpret_cast<const uint2*>((const uint8_t*)e.v + at);
-  x.m_scale = e.m_scale[at / kStateBlock];
-  x.r_scale = e.v_scale[at / kStateBlock];
+  x.m_scale = e.m_scale[threadIdx.x / 32];
+  x.r_scale = e.v_scale[threadIdx.x / 32];
 }
 
-// One thread's elements at `at`, fetched before where WHOLE.  All lanes of a
-// warp come here with the same WHOLE.
+// One thread's elements of a chunk, fetched before where WHOLE.  All lanes of a
+// warp, which hold one block of states, come here with the same WHOLE.
 template <bool WHOLE, typename P, typename G, bool MASTER, typename F>
-__device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f, const Betas& b, float eps,
-                                        float coef, int64_t at, const F& in) {
-  const int64_t left = e.n - at;
-  const int lane = threadIdx.x & 31;
-  if (!WHOLE && left + lane * kOptVec <= 0) return;  // no lane of the warp has elements
-  const int valid = WHOLE ? kOptVec : (int)max((int64_t)0, min((int64_t)kOptVec, left));
-  const int64_t block = at / kStateBlock;
+__device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float eps, float coef, const F& in) {
+  const unsigned at = threadIdx.x * kOptVec;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  if (!WHOLE && e.valid <= warp * kStateBlock) return;  // no lane of the warp has elements
+  const int valid = WHOLE ? kOptVec : max(0, min(kOptVec, e.valid - (int)at));
   P* p = (P*)e.param + at;
-  float* w = e.master + at;
+  float* w = (float*)e.weights + at;
   uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
   float xp[kOptVec], xg[kOptVec], xm[kOptVec], xr[kOptVec];
   uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
@@ -317,8 +363,8 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
         (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
       }
     }
-    m_scale = e.m_scale[block];
-    r_scale = e.v_scale[block];
+    m_scale = e.m_scale[warp];
+    r_scale = e.v_scale[warp];
   }
   codes_to_float(cm, xm);
   codes_to_float(cr, xr);
@@ -327,7 +373,7 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   // A sum of two products is a fused operation with a 1 that the compiler does
   // not know: it would make a packed product and sum one, with one rounding.
   const Two one = both(b.one);
-  const Two ki = both(-f.inv_sqrt), ke = both(eps), ks = both(-f.step), kd = both(f.decay);
+  const Two ki = both(-e.f.inv_sqrt), ke = both(eps), ks = both(-e.f.step), kd = both(e.f.decay);
   float m_top = 0.0f, r_top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kOptVec; i += 2) {
@@ -357,7 +403,7 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
   }
   float2 scale, inv;
   scales_of(m_top, r_top, scale, inv);
-  const uint32_t key = mix(f.key + (uint32_t)block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
+  const uint32_t key = mix(e.f.key + e.block + warp) + (uint32_t)lane * (kOptVec / 2 * kGolden);
   const Two im = both(inv.x), ir = both(-inv.y), grid = both(0x1p-120f);
   uint32_t code[kOptVec];
 #pragma unroll
@@ -365,14 +411,13 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
     const float2 qm = apart(two(xm[i], xm[i + 1]) * im);
     const float2 qr = apart(two(xr[i], xr[i + 1]) * ir * grid);
     const uint32_t word = mix(key + i / 2 * kGolden);
-    code[i] = round_stochastic(qr.x, xr[i], word & 0xFFFFu);
-    code[i + 1] = round_stochastic(qr.y, xr[i + 1], word >> 16);
+    code[i] = round_stochastic<0>(qr.x, xr[i], word);
+    code[i + 1] = round_stochastic<1>(qr.y, xr[i + 1], word);
     xm[i] = qm.x;
     xm[i + 1] = qm.y;
   }
   cm = float_to_codes(xm);
-  cr = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
-                  code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+  cr = make_uint2(top_bytes(code[0], code[1], code[2], code[3]), top_bytes(code[4], code[5], code[6], code[7]));
   if (WHOLE) {
     *reinterpret_cast<uint2*>(m) = cm;
     *reinterpret_cast<uint2*>(v) = cr;
@@ -386,27 +431,20 @@ __device__ __forceinline__ void update8(const AdamEntry& e, const AdamFactors& f
     }
   }
   if (lane == 0) {
-    e.m_scale[block] = scale.x;
-    e.v_scale[block] = scale.y;
+    e.m_scale[warp] = scale.x;
+    e.v_scale[warp] = scale.y;
   }
 }
 
-// What every block of a step begins with: each tensor's factors into shared
-// memory, the clipping factor.  False where the step is to change nothing.
-template <int CAP>
-__device__ __forceinline__ bool begin_step(const AdamTable<CAP>& tab, AdamFactors* factors, float& coef) {
-  const AdamHyper& h = tab.h;
-  for (int i = threadIdx.x; i < tab.count; i += kOptThreads) factors[i] = factors_of(tab.t[i], h);
+// The clipping factor, which every block of a step forms for itself.  False
+// where the step is to change nothing.
+__device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
   coef = 1.0f;
-  bool take = true;
-  if (h.part) {
-    const double norm = norm_of(h.part, h.parts);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
-    coef = clip_factor(norm, h.max_norm);
-    take = isfinite(norm);  // the same in every block
-  }
-  __syncthreads();
-  return take;
+  if (!h.part) return true;
+  const double norm = norm_of(h.part, h.parts);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
+  coef = clip_factor(norm, h.max_norm);
+  return isfinite(norm);  // the same in every block
 }
 
 // The last block to come here has every other block's reads of the clocks
@@ -415,6 +453,7 @@ template <int CAP>
 __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   const AdamHyper& h = tab.h;
   __shared__ bool s_last;
+  __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     s_last = atomicAdd(h.ticket, 1u) == gridDim.x - 1;
@@ -431,20 +470,22 @@ __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   if (threadIdx.x == 0) *h.ticket = 0;
 }
 
-__device__ __forceinline__ int64_t element_of(const AdamEntry& e, unsigned c) {
-  return (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
-}
-
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ AdamTable<CAP> tab) {
-  __shared__ AdamFactors s_factors[CAP];
+  __shared__ AdamSlot s_slots[kRounds][kOptWarps];
+  const unsigned warp = threadIdx.x / 32;
+  unsigned c = blockIdx.x;
+  look_up<P, G, MASTER, 32>(tab, c + warp * gridDim.x, s_slots[0][warp]);
   float coef;
-  if (!begin_step(tab, s_factors, coef)) return;
-  int i = tensor_of(tab.t, tab.count, blockIdx.x);
-  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    while (c >= tab.t[i].end_chunk) ++i;
-    const AdamEntry& e = tab.t[i];
-    update32<P, G, MASTER>(e, s_factors[i], tab.h.betas, tab.h.eps, coef, element_of(e, c));
+  if (!begin_step(tab.h, coef)) return;
+  __syncthreads();
+  for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
+    look_up<P, G, MASTER, 32>(tab, c + (kOptWarps + warp) * gridDim.x,
+                              s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+#pragma unroll 1
+    for (int b = 0; b < kOptWarps && c < tab.chunks; ++b, c += gridDim.x)
+      update32<P, G, MASTER>(s_slots[round][b], tab.h.betas, tab.h.eps, coef);
+    __syncthreads();
   }
   end_step(tab);
 }
@@ -454,32 +495,37 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
   using W = typename std::conditional<MASTER, float, P>::type;
-  __shared__ AdamFactors s_factors[CAP];
-  const auto whole_at = [&](const AdamEntry& e, int64_t at) { return e.aligned && (at | (kStateBlock - 1)) < e.n; };
-  const auto weights = [&](const AdamEntry& e) { return MASTER ? (const void*)e.master : e.param; };
-  int i = tensor_of(tab.t, tab.count, blockIdx.x);
-  int64_t at = element_of(tab.t[i], blockIdx.x);
-  bool whole = whole_at(tab.t[i], at);
-  Fetched<W, G> here, next;
-  if (whole) fetch(tab.t[i], weights(tab.t[i]), at, here);
+  __shared__ AdamSlot s_slots[kRounds][kOptWarps];
+  const int warp = threadIdx.x / 32;
+  const auto whole_in = [&](const AdamSlot& e) { return e.aligned && (warp + 1) * kStateBlock <= e.valid; };
+  unsigned c = blockIdx.x;
+  look_up<P, G, MASTER, 8>(tab, c + warp * gridDim.x, s_slots[0][warp]);
   float coef;
-  if (!begin_step(tab, s_factors, coef)) return;
-  for (unsigned c = blockIdx.x;;) {
-    const int this_i = i;
-    const int64_t this_at = at;
+  if (!begin_step(tab.h, coef)) return;
+  __syncthreads();
+  const AdamSlot* slot = &s_slots[0][0];
+  bool whole = whole_in(*slot);
+  Fetched<W, G> here, next;
+  if (whole) fetch(*slot, here);
+  for (int round = 0, b = 0;;) {
+    const AdamSlot* const this_slot = slot;
     const bool this_whole = whole;
     c += gridDim.x;
-    if (c < tab.chunks) {
-      while (c >= tab.t[i].end_chunk) ++i;
-      at = element_of(tab.t[i], c);
-      whole = whole_at(tab.t[i], at);
-      if (whole) fetch(tab.t[i], weights(tab.t[i]), at, next);
+    if (++b == kOptWarps) {
+      b = 0;
+      round = round + 1 == kRounds ? 0 : round + 1;
+      __syncthreads();  // the round was looked up
     }
-    const AdamEntry& e = tab.t[this_i];
-    if (this_whole)
-      update8<true, P, G, MASTER>(e, s_factors[this_i], tab.h.betas, tab.h.eps, coef, this_at, here);
-    else
-      update8<false, P, G, MASTER>(e, s_factors[this_i], tab.h.betas, tab.h.eps, coef, this_at, here);
+    if (c < tab.chunks) {
+      slot = &s_slots[round][b];
+      whole = whole_in(*slot);
+      if (whole) fetch(*slot, next);
+    }
+    if (b == 1)  // of the next round, whose chunk 0 is kOptWarps - 1 ahead
+      look_up<P, G, MASTER, 8>(tab, c + (kOptWarps - 1 + warp) * gridDim.x,
+                               s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+    if (this_whole) update8<true, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
+    else update8<false, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
     if (c >= tab.chunks) break;
     here = next;
   }
@@ -497,12 +543,14 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     for (; i < count && tab.count < CAP; ++i) {
       const dr_adamw_tensor& x = t[i];
       if (x.n == 0 || x.param_type != pt || x.grad_type != gt || (x.master != nullptr) != MASTER) continue;
-      const uintptr_t state = (uintptr_t)x.m | (uintptr_t)x.v;
-      const uintptr_t vectors = (uintptr_t)x.param | (uintptr_t)x.grad | (uintptr_t)x.master;
-      const int aligned = ((vectors & 15) | (state & (BITS == 32 ? 15 : 7))) == 0;
-      tab.t[tab.count++] = {x.param,   x.grad,     x.master,       x.m,    x.v,
-                            x.m_scale, x.v_scale,  x.clock,        x.n,    x.lr_ratio,
-                            x.weight_decay, x.seed, (unsigned)chunks, (unsigned)(chunks + opt_chunks(x.n)), aligned};
+      // m and v (8-bit: codes, eight bytes to a thread) are as long as floats (as codes).
+      const bool states = BITS == 32 ? vector_aligned((const float*)x.m) && vector_aligned((const float*)x.v)
+                                     : (((uintptr_t)x.m | (uintptr_t)x.v) & 7) == 0;
+      const int aligned = vector_aligned((const P*)x.param) && vector_aligned((const G*)x.grad) &&
+                          (!MASTER || vector_aligned(x.master)) && states;
+      tab.first[tab.count] = (unsigned)chunks;
+      tab.t[tab.count++] = {x.param, x.grad, x.master,   x.m,            x.v,    x.m_scale, x.v_scale,
+                            x.clock, x.n,    x.lr_ratio, x.weight_decay, x.seed, aligned};
       chunks += opt_chunks(x.n);
     }
     if (tab.count == 0) break;

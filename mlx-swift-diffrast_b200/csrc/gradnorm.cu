@@ -17,7 +17,6 @@ namespace {
 struct GradEntry {
   void* data;
   int64_t n;
-  unsigned first_chunk;
   int type;
 };
 
@@ -27,37 +26,113 @@ struct GradEntry {
 template <int CAP>
 struct GradTable {
   GradEntry t[CAP];
+  unsigned first[CAP];  // each tensor's first chunk
   int count;
   unsigned chunks;
 };
-constexpr int kSmall = 64, kLarge = 1280;
+constexpr int kSmall = 64, kLarge = 1000;
 static_assert(sizeof(GradTable<kLarge>) + 64 <= 32764, "kernel parameters");
 
 // Partial sums per launch at most, whatever the device.
 constexpr int kMaxParts = 2048;
 
+// A chunk: where it begins, how many elements of its tensor it holds.
+struct GradSlot {
+  char* data;
+  int valid, type;
+};
+
+template <int CAP>
+__device__ __forceinline__ void look_up(const GradTable<CAP>& tab, unsigned c, GradSlot& slot) {
+  if (c >= tab.chunks) return;
+  const int i = tensor_of(tab.first, tab.count, c);
+  const GradEntry& e = tab.t[i];
+  const int64_t at = (int64_t)(c - tab.first[i]) * kOptChunk;
+  if (threadIdx.x % 32 == 0)
+    slot = {(char*)e.data + at * (e.type == DR_F32 ? 4 : 2), (int)min((int64_t)kOptChunk, e.n - at), e.type};
+}
+
+// One thread's elements of a chunk, of any type, as they lie in memory.
+struct Fetched {
+  Words<float> w;  // a 16-bit type's elements are in the first half
+  int type;        // -1: nothing here, or summed already
+};
+
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const T* base, int64_t n, int64_t at) {
-  float x[kOptVec];
-  const T* p = base + at;
-  if (at + kOptVec <= n && ((uintptr_t)p & 15) == 0) load_vec(p, x);
-  else load_some(p, (int)max((int64_t)0, min((int64_t)kOptVec, n - at)), x);
+__device__ __forceinline__ double squares(const float (&x)[kOptVec]) {
   double s = 0.0;
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) s = __fma_rn((double)x[i], (double)x[i], s);
   return s;
 }
 
+template <typename T>
+__device__ __forceinline__ double squares_of(const T* p, int valid) {
+  float x[kOptVec];
+  load_some(p, valid, x);
+  return squares<T>(x);
+}
+
+// Fetches the thread's elements of a chunk, or, where they are not whole, adds
+// their squares to s.
+__device__ __forceinline__ void fetch(const GradSlot& e, Fetched& x, double& s) {
+  const int bytes = e.type == DR_F32 ? 4 : 2, valid = e.valid - (int)threadIdx.x * kOptVec;
+  const char* p = e.data + threadIdx.x * kOptVec * bytes;
+  x.type = -1;
+  if (valid >= kOptVec && (uintptr_t)p % (kOptVec * bytes) == 0) {
+    x.type = e.type;
+    if (e.type == DR_F32) x.w = load_words((const float*)p);
+    else x.w.w[0] = load_words((const __half*)p).w[0];
+  } else if (valid > 0) {
+    if (e.type == DR_F32) s += squares_of((const float*)p, valid);
+    else if (e.type == DR_BF16) s += squares_of((const __nv_bfloat16*)p, valid);
+    else s += squares_of((const __half*)p, valid);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ double squares_of(const Fetched& x) {
+  Words<T> w;
+#pragma unroll
+  for (int i = 0; i < Words<T>::kCount; ++i) w.w[i] = x.w.w[i];
+  float f[kOptVec];
+  widen_words(w, f);
+  return squares<T>(f);
+}
+
+// A thread's loads of kAhead chunks are under way together.
+constexpr int kAhead = 4;
+static_assert(kOptWarps % kAhead == 0, "rounds of whole batches");
+
 template <int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_constant__ GradTable<CAP> tab,
                                                                  double* __restrict__ part) {
+  __shared__ GradSlot s_slots[kRounds][kOptWarps];
+  const unsigned warp = threadIdx.x / 32;
   double s = 0.0;
-  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    const GradEntry& e = tab.t[tensor_of(tab.t, tab.count, c)];
-    const int64_t at = (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
-    if (e.type == DR_F32) s += chunk_squares((const float*)e.data, e.n, at);
-    else if (e.type == DR_BF16) s += chunk_squares((const __nv_bfloat16*)e.data, e.n, at);
-    else s += chunk_squares((const __half*)e.data, e.n, at);
+  unsigned c = blockIdx.x;
+  look_up(tab, c + warp * gridDim.x, s_slots[0][warp]);
+  __syncthreads();
+  for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
+#pragma unroll 1
+    for (int b = 0; b < kOptWarps && c < tab.chunks; b += kAhead) {
+      Fetched x[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        x[a].type = -1;
+        if (c < tab.chunks) fetch(s_slots[round][b + a], x[a], s);
+        c += gridDim.x;
+      }
+      if (b == 0)
+        look_up(tab, c + (kOptWarps - kAhead + warp) * gridDim.x, s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (x[a].type == DR_F32) s += squares_of<float>(x[a]);
+        else if (x[a].type == DR_BF16) s += squares_of<__nv_bfloat16>(x[a]);
+        else if (x[a].type == DR_F16) s += squares_of<__half>(x[a]);
+      }
+    }
+    __syncthreads();
   }
   s = block_sum(s);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -70,15 +145,16 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* 
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(T* base, int64_t n, int64_t at, float c) {
+__device__ __forceinline__ void scale_vec(const GradSlot& e, float f) {
+  const int valid = min(kOptVec, e.valid - (int)threadIdx.x * kOptVec);
+  if (valid <= 0) return;
   float x[kOptVec];
-  T* p = base + at;
-  const bool whole = at + kOptVec <= n && ((uintptr_t)p & 15) == 0;
-  const int valid = (int)max((int64_t)0, min((int64_t)kOptVec, n - at));
+  T* p = (T*)e.data + threadIdx.x * kOptVec;
+  const bool whole = valid == kOptVec && vector_aligned(p);
   if (whole) load_vec(p, x);
   else load_some(p, valid, x);
 #pragma unroll
-  for (int i = 0; i < kOptVec; ++i) x[i] = __fmul_rn(x[i], c);
+  for (int i = 0; i < kOptVec; ++i) x[i] = __fmul_rn(x[i], f);
   if (whole) store_vec(p, x);
   else store_some(p, valid, x);
 }
@@ -87,24 +163,31 @@ template <int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_clip_scale(const __grid_constant__ GradTable<CAP> tab,
                                                             const double* __restrict__ part, int parts,
                                                             double max_norm, float* __restrict__ norm) {
+  __shared__ GradSlot s_slots[kRounds][kOptWarps];
+  const unsigned warp = threadIdx.x / 32;
+  unsigned c = blockIdx.x;
+  look_up(tab, c + warp * gridDim.x, s_slots[0][warp]);
   const double s = norm_of(part, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
   const float f = clip_factor(s, max_norm);
   if (f == 1.0f) return;
-  for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    const GradEntry& e = tab.t[tensor_of(tab.t, tab.count, c)];
-    const int64_t at = (int64_t)(c - e.first_chunk) * kOptChunk + threadIdx.x * kOptVec;
-    if (e.type == DR_F32) chunk_scale((float*)e.data, e.n, at, f);
-    else if (e.type == DR_BF16) chunk_scale((__nv_bfloat16*)e.data, e.n, at, f);
-    else chunk_scale((__half*)e.data, e.n, at, f);
+  __syncthreads();
+  for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
+    look_up(tab, c + (kOptWarps + warp) * gridDim.x, s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+#pragma unroll 1
+    for (int b = 0; b < kOptWarps && c < tab.chunks; ++b, c += gridDim.x) {
+      const GradSlot& e = s_slots[round][b];
+      if (e.type == DR_F32) scale_vec<float>(e, f);
+      else if (e.type == DR_BF16) scale_vec<__nv_bfloat16>(e, f);
+      else scale_vec<__half>(e, f);
+    }
+    __syncthreads();
   }
 }
 
-// Blocks of a launch over `chunks`: enough to fill the device, and few enough
-// that adding their partial sums costs little.
-unsigned list_blocks(const dr_ctx* ctx, unsigned chunks) {
-  return std::max(1u, std::min(chunks, (unsigned)std::min(kMaxParts, ctx->num_sms * 8)));
-}
+// Blocks of a launch at most: enough to fill the device, and few enough that
+// adding their partial sums costs little.
+unsigned most_blocks(const dr_ctx* ctx) { return (unsigned)std::min(kMaxParts, ctx->num_sms * 4); }
 
 dr_status check_list(dr_ctx* ctx, const dr_grad_tensor* g, int count, const char* what) {
   DR_REQUIRE(ctx, count >= 0 && (count == 0 || g), "%s: null list or count < 0", what);
@@ -126,7 +209,8 @@ void fill(const dr_grad_tensor* g, int count, int* i, GradTable<CAP>* tab) {
   for (; *i < count && tab->count < CAP; ++*i) {
     const dr_grad_tensor& t = g[*i];
     if (t.n == 0) continue;
-    tab->t[tab->count++] = {t.data, t.n, (unsigned)chunks, t.type};
+    tab->first[tab->count] = (unsigned)chunks;
+    tab->t[tab->count++] = {t.data, t.n, t.type};
     chunks += opt_chunks(t.n);
   }
   tab->chunks = (unsigned)chunks;
@@ -138,7 +222,7 @@ dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* 
     GradTable<CAP> tab;
     fill(g, count, &i, &tab);
     if (tab.count == 0) break;
-    const unsigned blocks = list_blocks(ctx, tab.chunks);
+    const unsigned blocks = std::min(tab.chunks, most_blocks(ctx));
     DR_TB(ctx);
     k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work + *parts);
     DR_LAUNCHED(ctx, "grad_norm_parts");
@@ -154,8 +238,9 @@ dr_status launch_scale(dr_ctx* ctx, const dr_grad_tensor* g, int count, const do
     GradTable<CAP> tab;
     fill(g, count, &i, &tab);
     if (tab.count == 0) break;
+    const unsigned blocks = std::min(tab.chunks, 2 * most_blocks(ctx));
     DR_TB(ctx);
-    k_clip_scale<CAP><<<list_blocks(ctx, tab.chunks), kOptThreads, 0, ctx->stream>>>(tab, work, parts, max_norm, norm);
+    k_clip_scale<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work, parts, max_norm, norm);
     DR_LAUNCHED(ctx, "clip_scale");
   }
   return DR_OK;

@@ -35,18 +35,26 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return
 template <>
 __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
 
-// kOptVec consecutive elements as they lie in memory, at a 16-byte aligned address.
+// kOptVec consecutive elements as they lie in memory, at an address that is a
+// multiple of their size: one access of 16 or 32 bytes.
 template <typename T>
 struct Words {
   static constexpr int kCount = kOptVec * sizeof(T) / 16;
+  static_assert(kCount == 1 || kCount == 2, "16 or 32 bytes");
   uint4 w[kCount];
 };
 
 template <typename T>
 __device__ __forceinline__ Words<T> load_words(const T* p) {
   Words<T> x;
-#pragma unroll
-  for (int i = 0; i < Words<T>::kCount; ++i) x.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  if constexpr (Words<T>::kCount == 2)
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(x.w[0].x), "=r"(x.w[0].y), "=r"(x.w[0].z), "=r"(x.w[0].w), "=r"(x.w[1].x), "=r"(x.w[1].y),
+                   "=r"(x.w[1].z), "=r"(x.w[1].w)
+                 : "l"(p)
+                 : "memory");
+  else
+    x.w[0] = *reinterpret_cast<const uint4*>(p);
   return x;
 }
 
@@ -55,6 +63,15 @@ __device__ __forceinline__ void widen_words(const Words<T>& words, float (&x)[kO
   const T* e = reinterpret_cast<const T*>(words.w);
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) x[i] = widen(e[i]);
+}
+
+// The same from shared memory.
+template <typename T>
+__device__ __forceinline__ void shared_vec(const T* p, float (&x)[kOptVec]) {
+  Words<T> words;
+#pragma unroll
+  for (int i = 0; i < Words<T>::kCount; ++i) words.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  widen_words(words, x);
 }
 
 template <typename T>
@@ -68,8 +85,18 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[kOptVec]) {
   T* e = reinterpret_cast<T*>(words.w);
 #pragma unroll
   for (int i = 0; i < kOptVec; ++i) e[i] = narrow<T>(x[i]);
-#pragma unroll
-  for (int i = 0; i < Words<T>::kCount; ++i) reinterpret_cast<uint4*>(p)[i] = words.w[i];
+  if constexpr (Words<T>::kCount == 2)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(words.w[0].x),
+                 "r"(words.w[0].y), "r"(words.w[0].z), "r"(words.w[0].w), "r"(words.w[1].x), "r"(words.w[1].y),
+                 "r"(words.w[1].z), "r"(words.w[1].w)
+                 : "memory");
+  else
+    *reinterpret_cast<uint4*>(p) = words.w[0];
+}
+
+template <typename T>
+__host__ __device__ __forceinline__ bool vector_aligned(const T* p) {
+  return (uintptr_t)p % (kOptVec * sizeof(T)) == 0;
 }
 
 // `valid` (0 .. kOptVec) elements at any address of T's alignment; the others are 0.
@@ -92,16 +119,24 @@ inline int64_t opt_chunks(int64_t n) { return (n + kOptChunk - 1) / kOptChunk; }
 
 // The tensor of a list that chunk c belongs to: the last whose first chunk is
 // <= c.  Tensors without elements are not in the list, so it is the one.
-template <typename Entry>
-__device__ __forceinline__ int tensor_of(const Entry* t, int count, unsigned c) {
+__device__ __forceinline__ int tensor_of(const unsigned* first, int count, unsigned c) {
   int lo = 0, hi = count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t[mid].first_chunk <= c) lo = mid;
+    if (first[mid] <= c) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
+
+// A block takes chunks b, b + gridDim, ... in rounds of one to a warp: each
+// warp looks one chunk of the next round up and leaves what it found in shared
+// memory.  The list lies in the parameter bank, where each tensor's row is a
+// miss at its first use on a multiprocessor; eight warps wait for eight of them
+// at once.  Three rounds are kept: one being looked up, one in use, and one that
+// a slower warp may still be in.
+constexpr int kOptWarps = kOptThreads / 32;
+constexpr int kRounds = 3;
 
 // Sum over the block in a fixed order; every thread gets it.  kOptThreads threads.
 __device__ __forceinline__ double block_sum(double v) {
