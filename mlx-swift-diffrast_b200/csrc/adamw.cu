@@ -104,18 +104,24 @@ struct AdamSlot {
   uint32_t block;  // of states, from the tensor's first on
   int valid;       // elements
   int aligned;
+  int tensor;
 };
 
+// Chunk c into `slot`; `before`: what this warp looked up last (or nullptr).
 template <typename P, typename G, bool MASTER, int BITS, int CAP>
-__device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, AdamSlot& slot) {
+__device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, AdamSlot& slot,
+                                        const AdamSlot* before) {
   if (c >= tab.chunks) return;
   const int i = tensor_of(tab.first, tab.count, c);
   const AdamEntry& e = tab.t[i];
   const int64_t at = (int64_t)(c - tab.first[i]) * kOptChunk;
-  const AdamFactors f = factors_of(e, tab.h);
+  AdamFactors f;
+  if (before && before->tensor == i) f = before->f;
+  else f = factors_of(e, tab.h);
   if (threadIdx.x % 32 != 0) return;
   constexpr int kState = BITS == 32 ? 4 : 1;
   slot.f = f;
+  slot.tensor = i;
   slot.weights = MASTER ? (const void*)(e.master + at) : (const P*)e.param + at;
   slot.param = (P*)e.param + at;
   slot.grad = (const G*)e.grad + at;
@@ -475,13 +481,13 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
   __shared__ AdamSlot s_slots[kRounds][kOptWarps];
   const unsigned warp = threadIdx.x / 32;
   unsigned c = blockIdx.x;
-  look_up<P, G, MASTER, 32>(tab, c + warp * gridDim.x, s_slots[0][warp]);
+  look_up<P, G, MASTER, 32>(tab, c + warp * gridDim.x, s_slots[0][warp], nullptr);
   float coef;
   if (!begin_step(tab.h, coef)) return;
   __syncthreads();
   for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
     look_up<P, G, MASTER, 32>(tab, c + (kOptWarps + warp) * gridDim.x,
-                              s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+                              s_slots[round + 1 == kRounds ? 0 : round + 1][warp], &s_slots[round][warp]);
 #pragma unroll 1
     for (int b = 0; b < kOptWarps && c < tab.chunks; ++b, c += gridDim.x)
       update32<P, G, MASTER>(s_slots[round][b], tab.h.betas, tab.h.eps, coef);
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
   const int warp = threadIdx.x / 32;
   const auto whole_in = [&](const AdamSlot& e) { return e.aligned && (warp + 1) * kStateBlock <= e.valid; };
   unsigned c = blockIdx.x;
-  look_up<P, G, MASTER, 8>(tab, c + warp * gridDim.x, s_slots[0][warp]);
+  look_up<P, G, MASTER, 8>(tab, c + warp * gridDim.x, s_slots[0][warp], nullptr);
   float coef;
   if (!begin_step(tab.h, coef)) return;
   __syncthreads();
@@ -507,13 +513,14 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
   bool whole = whole_in(*slot);
   Fetched<W, G> here, next;
   if (whole) fetch(*slot, here);
-  for (int round = 0, b = 0;;) {
+  for (int round = 0, following = 1, b = 0;;) {
     const AdamSlot* const this_slot = slot;
     const bool this_whole = whole;
     c += gridDim.x;
     if (++b == kOptWarps) {
       b = 0;
-      round = round + 1 == kRounds ? 0 : round + 1;
+      round = following;
+      if (++following == kRounds) following = 0;
       __syncthreads();  // the round was looked up
     }
     if (c < tab.chunks) {
@@ -521,9 +528,9 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
       whole = whole_in(*slot);
       if (whole) fetch(*slot, next);
     }
-    if (b == 1)  // of the next round, whose chunk 0 is kOptWarps - 1 ahead
-      look_up<P, G, MASTER, 8>(tab, c + (kOptWarps - 1 + warp) * gridDim.x,
-                               s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
+    if (b == 1)  // the next round, whose chunk 0 is kOptWarps - 1 ahead
+      look_up<P, G, MASTER, 8>(tab, c + (kOptWarps - 1 + warp) * gridDim.x, s_slots[following][warp],
+                               &s_slots[round][warp]);
     if (this_whole) update8<true, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
     else update8<false, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
     if (c >= tab.chunks) break;
