@@ -447,6 +447,7 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
 __device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
   coef = 1.0f;
   if (!h.part) return true;
+  after_previous();
   const double norm = norm_of(h.part, h.parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
   coef = clip_factor(norm, h.max_norm);
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
 
 // One launch for the tensors of one combination of types, CAP at a time.
 template <typename P, typename G, bool MASTER, int BITS, int CAP>
-dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyper& h, int pt, int gt) {
+dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyper& h, int pt, int gt, bool* early) {
   for (int i = 0; i < count;) {
     AdamTable<CAP> tab;
     int64_t chunks = 0;
@@ -562,17 +563,26 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     }
     if (tab.count == 0) break;
     tab.chunks = (unsigned)chunks;
+    // Behind the norm's launch: while it is still running.
+    const auto start = [&](void (*kernel)(AdamTable<CAP>), unsigned blocks) {
+      if (*early) {
+        *early = false;
+        return launch_early(ctx->stream, blocks, kernel, tab);
+      }
+      kernel<<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+      return cudaSuccess;
+    };
     DR_TB(ctx);
     if (BITS == 32) {
-      const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 8);
-      k_adamw<P, G, MASTER, CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+      const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 4);
+      DR_CUDA(ctx, start(k_adamw<P, G, MASTER, CAP>, blocks), "adamw");
     } else {
       auto* kernel = k_adamw8<P, G, MASTER, CAP>;
       // One wave of blocks that stay.
       int resident = 0;
       DR_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kOptThreads, 0), "adamw8");
       const unsigned blocks = std::min(tab.chunks, (unsigned)(ctx->num_sms * std::max(resident, 1)));
-      kernel<<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+      DR_CUDA(ctx, start(kernel, blocks), "adamw8");
     }
     DR_LAUNCHED(ctx, BITS == 32 ? "adamw" : "adamw8");
   }
@@ -581,16 +591,16 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
 
 template <typename P, typename G, bool MASTER>
 dr_status launch_types(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyper& h, int bits, int pt,
-                       int gt) {
+                       int gt, bool* early) {
   int members = 0;
   for (int i = 0; i < count; ++i)
     members += t[i].n != 0 && t[i].param_type == pt && t[i].grad_type == gt && (t[i].master != nullptr) == MASTER;
   if (members == 0) return DR_OK;
   if (members <= kSmall)
-    return bits == 32 ? launch<P, G, MASTER, 32, kSmall>(ctx, t, count, h, pt, gt)
-                      : launch<P, G, MASTER, 8, kSmall>(ctx, t, count, h, pt, gt);
-  return bits == 32 ? launch<P, G, MASTER, 32, kLarge>(ctx, t, count, h, pt, gt)
-                    : launch<P, G, MASTER, 8, kLarge>(ctx, t, count, h, pt, gt);
+    return bits == 32 ? launch<P, G, MASTER, 32, kSmall>(ctx, t, count, h, pt, gt, early)
+                      : launch<P, G, MASTER, 8, kSmall>(ctx, t, count, h, pt, gt, early);
+  return bits == 32 ? launch<P, G, MASTER, 32, kLarge>(ctx, t, count, h, pt, gt, early)
+                    : launch<P, G, MASTER, 8, kLarge>(ctx, t, count, h, pt, gt, early);
 }
 
 }  // namespace
@@ -638,15 +648,16 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
     dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
     if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);
     for (int i = 0; i < count; ++i) g[i] = {const_cast<void*>(t[i].grad), t[i].n, t[i].grad_type, 0};
-    const dr_status st = grad_norm_parts(ctx, g, count, (double*)work, &h.parts);
+    const dr_status st = grad_norm_parts(ctx, g, count, (double*)work, &h.parts, nullptr);
     delete[] g;
     if (st != DR_OK) return st;
     h.part = (const double*)work;
     if (h.parts == 0) return grad_norm_finish(ctx, (const double*)work, 0, norm);
   }
+  bool early = h.part != nullptr;
 #define DR_ADAMW(P, G, MASTER, PT, GT)                                                                  \
   do {                                                                                                  \
-    const dr_status st = launch_types<P, G, MASTER>(ctx, t, count, h, state_bits, PT, GT);              \
+    const dr_status st = launch_types<P, G, MASTER>(ctx, t, count, h, state_bits, PT, GT, &early);              \
     if (st != DR_OK) return st;                                                                         \
   } while (0)
   DR_ADAMW(float, float, false, DR_F32, DR_F32);

@@ -106,7 +106,8 @@ static_assert(kOptWarps % kAhead == 0, "rounds of whole batches");
 
 template <int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_constant__ GradTable<CAP> tab,
-                                                                 double* __restrict__ part) {
+                                                                 double* __restrict__ part,
+                                                                 float* __restrict__ norm) {
   __shared__ GradSlot s_slots[kRounds][kOptWarps];
   const unsigned warp = threadIdx.x / 32;
   double s = 0.0;
@@ -134,12 +135,16 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_co
     }
     __syncthreads();
   }
+  let_next_start();
   s = block_sum(s);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
+  if (threadIdx.x != 0) return;
+  if (norm) *norm = (float)sqrt(s);  // the only block of the only launch
+  else part[blockIdx.x] = s;
 }
 
 __global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* __restrict__ part, int count,
                                                                   float* __restrict__ norm) {
+  after_previous();
   const double s = norm_of(part, count);
   if (threadIdx.x == 0) *norm = (float)s;
 }
@@ -167,6 +172,7 @@ __global__ void __launch_bounds__(kOptThreads) k_clip_scale(const __grid_constan
   const unsigned warp = threadIdx.x / 32;
   unsigned c = blockIdx.x;
   look_up(tab, c + warp * gridDim.x, s_slots[0][warp]);
+  after_previous();
   const double s = norm_of(part, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
   const float f = clip_factor(s, max_norm);
@@ -217,14 +223,14 @@ void fill(const dr_grad_tensor* g, int count, int* i, GradTable<CAP>* tab) {
 }
 
 template <int CAP>
-dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* work, int* parts) {
+dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* work, int* parts, float* norm) {
   for (int i = 0; i < count;) {
     GradTable<CAP> tab;
     fill(g, count, &i, &tab);
     if (tab.count == 0) break;
-    const unsigned blocks = std::min(tab.chunks, most_blocks(ctx));
+    const unsigned blocks = norm ? 1 : std::min(tab.chunks, most_blocks(ctx));
     DR_TB(ctx);
-    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work + *parts);
+    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work + *parts, norm);
     DR_LAUNCHED(ctx, "grad_norm_parts");
     *parts += (int)blocks;
   }
@@ -234,13 +240,18 @@ dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* 
 template <int CAP>
 dr_status launch_scale(dr_ctx* ctx, const dr_grad_tensor* g, int count, const double* work, int parts,
                        double max_norm, float* norm) {
+  bool first = true;  // the launch behind the norm's
   for (int i = 0; i < count;) {
     GradTable<CAP> tab;
     fill(g, count, &i, &tab);
     if (tab.count == 0) break;
     const unsigned blocks = std::min(tab.chunks, 2 * most_blocks(ctx));
     DR_TB(ctx);
-    k_clip_scale<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work, parts, max_norm, norm);
+    if (first)
+      DR_CUDA(ctx, launch_early(ctx->stream, blocks, k_clip_scale<CAP>, tab, work, parts, max_norm, norm), "clip_scale");
+    else
+      k_clip_scale<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work, parts, max_norm, norm);
+    first = false;
     DR_LAUNCHED(ctx, "clip_scale");
   }
   return DR_OK;
@@ -250,15 +261,16 @@ dr_status launch_scale(dr_ctx* ctx, const dr_grad_tensor* g, int count, const do
 
 dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* norm) {
   DR_TB(ctx);
-  k_grad_norm_finish<<<1, kOptThreads, 0, ctx->stream>>>(work, parts, norm);
+  DR_CUDA(ctx, launch_early(ctx->stream, 1, k_grad_norm_finish, work, parts, norm), "grad_norm_finish");
   DR_LAUNCHED(ctx, "grad_norm_finish");
   return DR_OK;
 }
 
-dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts) {
+dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts,
+                          float* norm) {
   *parts = 0;
-  return count <= kSmall ? launch_parts<kSmall>(ctx, grads, count, work, parts)
-                         : launch_parts<kLarge>(ctx, grads, count, work, parts);
+  return count <= kSmall ? launch_parts<kSmall>(ctx, grads, count, work, parts, norm)
+                         : launch_parts<kLarge>(ctx, grads, count, work, parts, norm);
 }
 
 }  // namespace dr
@@ -277,8 +289,12 @@ dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, floa
   DR_REQUIRE(ctx, norm && work && ((uintptr_t)work & 7) == 0, "grad_norm: norm and an 8-byte aligned work are required");
   dr_status st = check_list(ctx, grads, count, "grad_norm");
   if (st != DR_OK) return st;
+  // The whole of a list of one block is formed in its one launch.
   int parts = 0;
-  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts)) != DR_OK) return st;
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) chunks += opt_chunks(grads[i].n);
+  const bool one = chunks > 0 && chunks <= kOptWarps && count <= kSmall;
+  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, one ? norm : nullptr)) != DR_OK || one) return st;
   return grad_norm_finish(ctx, (const double*)work, parts, norm);
 }
 
@@ -291,7 +307,7 @@ dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count,
   dr_status st = check_list(ctx, grads, count, "clip_grad_norm");
   if (st != DR_OK) return st;
   int parts = 0;
-  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts)) != DR_OK) return st;
+  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, nullptr)) != DR_OK) return st;
   if (parts == 0) return grad_norm_finish(ctx, (const double*)work, 0, norm);  // nothing to scale
   return count <= kSmall ? launch_scale<kSmall>(ctx, grads, count, (const double*)work, parts, max_norm, norm)
                          : launch_scale<kLarge>(ctx, grads, count, (const double*)work, parts, max_norm, norm);

@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <utility>
+
 #include "common.cuh"
 
 namespace dr {
@@ -166,9 +168,30 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
   return c >= 1.0 ? 1.0f : (float)c;
 }
 
+// Launches `kernel`, which calls after_previous(), while the launch before it on
+// the stream is still running.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(cudaStream_t stream, unsigned blocks, void (*kernel)(Params...), Args&&... args) {
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(kOptThreads);
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
+// In a kernel that the next one on the stream may overlap: it may start.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// In a kernel launched early: what the launch before it wrote is there.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 bool valid_type(int type);
 // Launches the partial sums of squares of a list; *parts of them lie in `work`.
-dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts);
+// With `norm`, for a list of one launch: one block forms the norm itself.
+dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts, float* norm);
 // *norm = the norm that the partial sums give.
 dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* norm);
 

@@ -7,6 +7,7 @@ in fp32, bf16 or fp16, AdamW's states in 32 or in 8 bits.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Sequence, Union
 
@@ -124,8 +125,13 @@ def _context(index: int):
     return c
 
 
-def _norm_work(c, count: int, dev) -> torch.Tensor:
-    return torch.empty(int(L.lib().dr_grad_norm_work_bytes(c, count)) // 8, dtype=torch.float64, device=dev)
+@functools.lru_cache(maxsize=256)
+def _work_len(index: int, count: int) -> int:
+    return int(L.lib().dr_grad_norm_work_bytes(L.ctx_for(index), count)) // 8
+
+
+def _norm_work(index: int, count: int) -> torch.Tensor:
+    return torch.empty(_work_len(index, count), dtype=torch.float64, device=_CUDA[index])
 
 
 def _norm_call(fn, ts, what: str, apart: bool, dense, *args) -> torch.Tensor:
@@ -145,7 +151,7 @@ def _norm_call(fn, ts, what: str, apart: bool, dense, *args) -> torch.Tensor:
     # From torch's allocator at each call: both belong to the stream (or to the
     # graph being captured) and to no other call.
     norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
-    work = _norm_work(c, len(ts), _CUDA[index])
+    work = _norm_work(index, len(ts))
     status = fn(c, rows, len(ts), *args, norm.data_ptr(), work.data_ptr())
     if status:
         L.check(status, c, what)
@@ -292,7 +298,7 @@ class AdamW:
         self._index, self._device = dev.index, dev
         with torch.cuda.device(dev):
             # A step's own: steps of one optimizer never run side by side.
-            self._work = _norm_work(_context(dev.index), count, dev)
+            self._work = _norm_work(dev.index, count)
         self._ticket_at, self._work_at = self._ticket.data_ptr(), self._work.data_ptr()
         # What a step's gradients are held against.
         self._shapes = [p.shape for p in self.params]
