@@ -559,7 +559,8 @@ typedef struct dr_adamw_tensor {
  *   g = coef * grad
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr wd) - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * and clock advances to t.  lr = lr_ratio * (*lr_device, a device float read by
+ * and clock advances to t (state_bits = 8: the quotient is within two units in
+ * the last place, and a v below 2^-100 loses bits).  eps is 2^-126 at least.  lr = lr_ratio * (*lr_device, a device float read by
  * the step, or `lr` when lr_device is NULL).
  * max_norm > 0: coef = min(1, max_norm / (norm + 1e-6)) with *norm (device, out)
  * the norm over the step's gradients, `work` as for dr_grad_norm; a step whose
@@ -573,7 +574,9 @@ typedef struct dr_adamw_tensor {
  * 2^-9 * scale at least.
  * ticket: device uint32, 0 before the first step that uses it, and 0 again
  * after each; steps that may overlap on the GPU need tickets of their own.
- * Tensors must not overlap.  `tensors` is a host array, read before the call
+ * Tensors must not overlap, nor gradients other tensors' parameters.  Any
+ * alignment of the element types is accepted; whole vectors are used where every
+ * pointer of a tensor is a multiple of 8 elements.  `tensors` is a host array, read before the call
  * returns; the step reads nothing back and can be captured in a CUDA graph, a
  * replay being the next step. */
 DR_API dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* tensors, int count, double lr,

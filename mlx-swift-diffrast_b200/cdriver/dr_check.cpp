@@ -8,6 +8,8 @@
 //   * antialias: a constant colour is returned unchanged;
 //   * the VJPs run and leave finite gradients; dr_ctx_sync reports no error;
 //   * the fused two-layer pass's one-pass VJP equals the separate VJPs;
+//   * the gradient norm, clipping and AdamW (32-bit and 8-bit states) of two
+//     small tensors against host arithmetic;
 //   * misuse returns DR_EINVAL with a message instead of crashing.
 // Exit status 0 when every check passes.
 #include <cuda_runtime.h>
@@ -191,6 +193,77 @@ int main() {
                     (void*)o[1], (void*)od[0], (void*)od[1], (void*)dg, (void*)fa, (void*)fv, (void*)sa, (void*)sr,
                     (void*)sv})
       cudaFree(p);
+  }
+
+  // gradient norm, clipping and two AdamW steps over two tensors, of which the
+  // second begins one element off a vector's alignment
+  {
+    const int n[2] = {300, 7};
+    std::vector<float> p0(308), g0(308);
+    for (size_t k = 0; k < p0.size(); ++k) {
+      p0[k] = std::sin(0.37f * (float)k);
+      g0[k] = 0.01f * std::cos(1.1f * (float)k);
+    }
+    const size_t at[2] = {0, 301};
+    double sum = 0.0;
+    for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < n[i]; ++k) sum += (double)g0[at[i] + k] * g0[at[i] + k];
+    const double norm0 = std::sqrt(sum), max_norm = 0.5 * norm0, coef = max_norm / (norm0 + 1e-6);
+    float* d_norm = dev(std::vector<float>(1, 0.0f));
+    unsigned char* d_work = dev(std::vector<unsigned char>(dr_grad_norm_work_bytes(ctx, 2)));
+    uint32_t* d_ticket = dev(std::vector<uint32_t>(1, 0u));
+    for (int bits : {32, 8}) {
+      float *d_p = dev(p0), *d_g = dev(g0);
+      unsigned char *d_m = dev(std::vector<unsigned char>(4 * 1024)), *d_v = dev(std::vector<unsigned char>(4 * 1024));
+      float *d_ms = dev(std::vector<float>(4)), *d_vs = dev(std::vector<float>(4));
+      double* d_clock = dev(std::vector<double>{0.0, 1.0, 1.0, 0.0, 0.0, 1.0, 1.0, 0.0});
+      cudaMemset(d_m, 0, 4096);
+      cudaMemset(d_v, 0, 4096);
+      cudaMemset(d_ms, 0, 16);
+      cudaMemset(d_vs, 0, 16);
+      dr_grad_tensor gt[2];
+      dr_adamw_tensor at_[2];
+      for (int i = 0; i < 2; ++i) {
+        const size_t slot = i ? 512 : 0, bytes = slot * (bits / 8);
+        gt[i] = {d_g + at[i], n[i], DR_F32, 0};
+        at_[i] = {d_p + at[i], d_g + at[i], nullptr, d_m + bytes, d_v + bytes, d_ms + slot / 256, d_vs + slot / 256,
+                  d_clock + 4 * i, n[i], 1.0, 0.1, (uint32_t)i, DR_F32, DR_F32, 0};
+      }
+      OK(dr_grad_norm(ctx, gt, 2, d_norm, d_work));
+      OK(dr_ctx_sync(ctx));
+      CHECK(std::fabs(host(d_norm, 1)[0] - norm0) <= 1e-6 * norm0, "norm %g, %g expected", host(d_norm, 1)[0], norm0);
+      // step 1 clips inside; then the gradients are clipped in place and step 2 takes them
+      OK(dr_adamw_step(ctx, at_, 2, 0.01, nullptr, 0.9, 0.999, 1e-8, bits, max_norm, d_norm, d_work, d_ticket));
+      OK(dr_clip_grad_norm(ctx, gt, 2, max_norm, d_norm, d_work));
+      OK(dr_adamw_step(ctx, at_, 2, 0.01, nullptr, 0.9, 0.999, 1e-8, bits, 0.0, nullptr, nullptr, d_ticket));
+      OK(dr_ctx_sync(ctx));
+      const std::vector<float> p = host(d_p, 308), g = host(d_g, 308);
+      const std::vector<double> clock = host(d_clock, 8);
+      double worst = 0.0;
+      for (int i = 0; i < 2; ++i) {
+        CHECK(clock[4 * i] == 2.0 && std::fabs(clock[4 * i + 1] - 0.81) < 1e-12, "clock %d at %g", i, clock[4 * i]);
+        for (int k = 0; k < n[i]; ++k) {
+          const double gk = coef * g0[at[i] + k];
+          CHECK(std::fabs(g[at[i] + k] - gk) <= 1e-6 * std::fabs(gk), "clipped gradient %d", k);
+          double w = p0[at[i] + k], m = 0.0, v = 0.0;
+          for (int t = 1; t <= 2; ++t) {
+            m = 0.9 * m + 0.1 * gk;
+            v = 0.999 * v + 0.001 * gk * gk;
+            w = w * (1 - 0.01 * 0.1) - 0.01 / (1 - std::pow(0.9, t)) * m /
+                                           (std::sqrt(v) / std::sqrt(1 - std::pow(0.999, t)) + 1e-8);
+          }
+          worst = std::fmax(worst, std::fabs(p[at[i] + k] - w));
+        }
+      }
+      // a state of 3 bits behind the leading one is up to 1/8 off, in the second of two steps of 0.01
+      CHECK(worst <= (bits == 32 ? 1e-6 : 0.01 * 0.35), "AdamW, %d bits: %g off", bits, worst);
+      CHECK(p[300] == p0[300], "the element between the tensors was written");
+      for (void* q : {(void*)d_p, (void*)d_g, (void*)d_m, (void*)d_v, (void*)d_ms, (void*)d_vs, (void*)d_clock})
+        cudaFree(q);
+    }
+    CHECK(dr_adamw_step(ctx, nullptr, 1, 0.01, nullptr, 0.9, 0.999, 1e-8, 32, 0.0, nullptr, nullptr, d_ticket) ==
+              DR_EINVAL, "a null list was taken");
+    for (void* q : {(void*)d_norm, (void*)d_work, (void*)d_ticket}) cudaFree(q);
   }
 
   // misuse is a status, not a crash

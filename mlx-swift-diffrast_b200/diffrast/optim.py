@@ -15,7 +15,11 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from . import _rows
+try:
+    from . import _rows
+except ImportError as e:
+    raise ImportError("diffrast/_rows.so is missing or of another Python or torch; build it with "
+                      f"`python mlx-swift-diffrast_b200/build.py` ({e})") from e
 from .ops import _ctx, _f32, _ptr
 
 
@@ -118,6 +122,14 @@ def _grad_table(ts):
     return tab
 
 
+def _written(ts) -> None:
+    """Tells autograd that the tensors were changed in place (inference tensors do not count changes)."""
+    try:
+        torch.autograd.graph.increment_version(ts)
+    except RuntimeError:
+        torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
+
+
 def _context(index: int):
     """The context of a device, on torch's current stream there."""
     c = L.ctx_for(index)
@@ -184,7 +196,7 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
         return t
 
     norm = _norm_call(L.lib().dr_clip_grad_norm, ts, "clip_grad_norm_", True, dense, max_norm)
-    torch.autograd.graph.increment_version(ts)
+    _written(ts)
     return norm
 
 
@@ -355,7 +367,8 @@ class AdamW:
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Optional[torch.Tensor]:
         """One step from `grads` (one for each parameter, or None to leave it as
         it is; default: the parameters' .grad).  Gradients have their parameter's
-        shape and type, or one of the two is float32.  Returns the norm of the
+        shape and type, or one of the two is float32; they share no memory with
+        other parameters.  Returns the norm of the
         gradients (a float32 scalar on the device) with max_grad_norm, else None."""
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self._index):
@@ -385,7 +398,7 @@ class AdamW:
             self._work_at, self._ticket_at)
         if status:
             L.check(status, c, "AdamW")
-        torch.autograd.graph.increment_version(at)
+        _written(at)
         return norm
 
     def moments(self, i: int):

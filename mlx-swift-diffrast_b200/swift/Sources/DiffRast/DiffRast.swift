@@ -598,6 +598,40 @@ public enum DiffRast {
                                eps, c1, c2), "adamStep")
     }
 
+    public typealias GradTensor = dr_grad_tensor
+    public typealias AdamWTensor = dr_adamw_tensor
+
+    /// A gradient of `type` (DR_F32, DR_BF16 or DR_F16) for gradNorm / clipGradNorm.
+    public static func gradient(_ g: DeviceTensor, type: dr_dtype = DR_F32) -> GradTensor {
+        GradTensor(data: g.pointer, n: Int64(g.count), type: Int32(type.rawValue), reserved: 0)
+    }
+
+    /// The 2-norm over all gradients, into the device scalar `norm`; `work` holds gradNormWorkBytes.
+    public static func gradNorm(_ ctx: Context, _ grads: [GradTensor], norm: DeviceTensor, work: DeviceTensor) {
+        ctx.check(dr_grad_norm(ctx.raw, grads, Int32(grads.count), norm.f, work.pointer), "gradNorm")
+    }
+
+    /// gradNorm, then the gradients times min(1, maxNorm / (norm + 1e-6)) in place.
+    public static func clipGradNorm(_ ctx: Context, _ grads: [GradTensor], maxNorm: Double, norm: DeviceTensor,
+                                    work: DeviceTensor) {
+        ctx.check(dr_clip_grad_norm(ctx.raw, grads, Int32(grads.count), maxNorm, norm.f, work.pointer),
+                  "clipGradNorm")
+    }
+
+    public static func gradNormWorkBytes(_ ctx: Context, count: Int) -> Int {
+        Int(dr_grad_norm_work_bytes(ctx.raw, Int32(count)))
+    }
+
+    /// One AdamW step over many tensors (rows as the header describes them), states in 32 or 8 bits; with maxNorm
+    /// the gradients are clipped by their norm, which lands in `norm`.
+    public static func adamwStep(_ ctx: Context, _ tensors: [AdamWTensor], lr: Double, beta1: Double = 0.9,
+                                 beta2: Double = 0.999, eps: Double = 1e-8, stateBits: Int = 32,
+                                 maxNorm: Double = 0, norm: DeviceTensor? = nil, work: DeviceTensor? = nil,
+                                 ticket: UnsafeMutablePointer<UInt32>, lrDevice: DeviceTensor? = nil) {
+        ctx.check(dr_adamw_step(ctx.raw, tensors, Int32(tensors.count), lr, lrDevice?.f, beta1, beta2, eps,
+                                Int32(stateBits), maxNorm, norm?.f, work?.pointer, ticket), "adamwStep")
+    }
+
     /// Allocation-free topology hash (fixed table in the library, at most
     /// DR_STATIC_TOPO_MAX_TRIS triangles): writes `topo` [T, 3].
     public static func antialiasConstructTopologyHashStatic(tri: DeviceTensor, topo: DeviceTensor,

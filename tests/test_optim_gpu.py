@@ -524,3 +524,179 @@ def test_a_training_step_from_render_to_update():
             by_hand.step(clipped)
         for a, b in zip(params, by_hand.params):
             assert torch.equal(a.detach(), b)
+
+
+# ---------------------------------------------------------- calls in the wild
+
+def unfused8(state, g, coef, seeds, begins, counts, t):
+    """8-bit states after a step, each operation a torch one in float32: (m, r, scales) of each tensor."""
+    out = []
+    for b, n, seed in zip(begins, counts, seeds):
+        pad = -(-n // 256) * 256
+        gi = torch.zeros(pad, device="cuda")
+        gi[:n] = g[b:b + n].float()
+        if coef is not None:
+            gi = gi * coef
+        m, r = (state[k][b:b + pad].float().view(-1, 256) * state[k + "_scale"][b // 256:(b + pad) // 256, None]
+                for k in ("m", "r"))
+        m = (m * 0.9).view(-1) + gi * (1 - 0.9)
+        r = ((r * r * 0.999).view(-1) + gi * gi * (1 - 0.999)).sqrt()
+        res = []
+        for x in (m, r):
+            x = x.view(-1, 256)
+            top = x.abs().amax(1)
+            inv = torch.where(top > 0, torch.full_like(top, 448.0) / top, 0.0)
+            res += [(x * inv[:, None]).view(-1), top * (1 / 448)]
+        bits = torch.from_numpy(AO.random16(pad, seed, t)).to("cuda", torch.int32)
+        y = torch.where(res[2] > 0, res[2].clamp_min(2.0 ** -9), 0.0)
+        low = torch.where(y < 2.0 ** -6, 2.0 ** -6, 0.0)
+        y = (((y + low).view(torch.int32) + bits * 16 + 8) & ~0xFFFFF).view(torch.float32) - low
+        out.append((res[0].clamp(-448, 448).to(torch.float8_e4m3fn).float()[:n], y.clamp(max=448.0)[:n], res[1], res[3]))
+    return out
+
+
+@pytest.mark.parametrize("g_type", [F32, F16])
+def test_adamw8_codes_are_the_unfused_evaluations(g_type):
+    # Codes and scales bit for bit, over several steps: no rounding is left out and none is added.
+    rng = np.random.default_rng(19)
+    counts = [100_000, 777, 3]
+    params = [torch.randn(n, device="cuda").to(g_type) for n in counts]
+    opt = optim.AdamW(params, state_bits=8, max_grad_norm=0.5, seed=11)
+    begins = [int(b) for b in opt._begins]
+    flat = torch.zeros(opt.state["m"].numel(), device="cuda", dtype=g_type)
+    for t in range(1, 6):
+        gs = [grads_like(rng, n, g_type) for n in counts]
+        for b, g in zip(begins, gs):
+            flat[b:b + g.numel()] = g
+        norm = torch.stack([g.double().square().sum() for g in gs]).sum().sqrt()
+        coef = (0.5 / (norm + 1e-6)).clamp(max=1.0).float()
+        want = unfused8(opt.state, flat, coef, [int(x) for x in opt._tab["seed"]], begins, counts, t)
+        opt.step(gs)
+        for i, (m, r, ms, rs) in enumerate(want):
+            assert torch.equal(opt._flat("m", i).float(), m) and torch.equal(opt._flat("r", i).float(), r)
+            assert torch.equal(opt._flat("m_scale", i), ms) and torch.equal(opt._flat("r_scale", i), rs)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_queued_steps_are_the_waited_ones(bits):
+    # 60 clipped steps queued without a wait, their gradients made by kernels between them, against the same steps
+    # with a wait after each launch: the step that begins while the norm still runs reads nothing too early.
+    def run(wait):
+        torch.manual_seed(4)
+        params = [torch.randn(n, device="cuda") for n in (400_000, 31, 70_003)]
+        opt = optim.AdamW(params, state_bits=bits, max_grad_norm=1.0, learning_rate=1e-2)
+        norms = []
+        for _ in range(60):
+            gs = [torch.sin(p * 3) * 0.1 for p in params]
+            if wait:
+                torch.cuda.synchronize()
+            norms.append(opt.step(gs))
+            if wait:
+                torch.cuda.synchronize()
+            optim.clip_grad_norm_(gs, 0.01)
+            norms.append(optim.grad_norm(gs))
+        torch.cuda.synchronize()
+        return params, norms
+    (p1, n1), (p2, n2) = run(False), run(True)
+    assert all(torch.equal(a, b) for a, b in zip(p1, p2)) and torch.equal(torch.stack(n1), torch.stack(n2))
+
+
+def test_clip_of_more_tensors_than_a_launch_carries():
+    rng = np.random.default_rng(21)
+    gs = [grads_like(rng, int(rng.integers(1, 400)), (F32, BF16, F16)[i % 3]) for i in range(2300)]
+    old = [f64(g) for g in gs]
+    ref = math.sqrt(sum(float((x ** 2).sum()) for x in old))
+    got = optim.clip_grad_norm_(gs, 0.25 * ref)
+    assert abs(float(got) - ref) <= 1.01 * AO.U * ref
+    c = AO.clip_factor(ref, 0.25 * ref)
+    for g, x in zip(gs, old):
+        y = x * c
+        assert np.all(np.abs(f64(g) - y) <= (2 * AO.U + HALF[g.dtype]) * np.abs(y) * (1 + 4 * AO.U) + 2.0 ** -25)
+
+
+def test_modules_parameters_inference_tensors_and_generators():
+    lin = torch.nn.Linear(17, 5).cuda()
+    opt = optim.AdamW(lin.parameters(), learning_rate=0.01, max_grad_norm=1.0)
+    lin(torch.randn(3, 17, device="cuda")).sum().backward()
+    before = [p.detach().clone() for p in lin.parameters()]
+    run_steps(opt, lambda: [p.grad for p in lin.parameters()], steps=1)
+    assert all(not torch.equal(a, b) for a, b in zip(before, lin.parameters()))
+    with torch.inference_mode():
+        x = torch.ones(9, device="cuda")
+        y = torch.zeros(9, device="cuda")
+        inner = optim.AdamW([y], learning_rate=0.1)
+        inner.step([x])
+        assert float(optim.clip_grad_norm_((t for t in [x]), 1.5)) == 3.0
+    torch.testing.assert_close(x.cpu(), torch.full((9,), 0.5), rtol=1e-6, atol=0)
+    assert (y < -0.09).all()
+
+
+def test_state_stays_where_it_is_while_a_graph_lives():
+    # A captured step, an eager one between its replays, a state loaded between them: one sequence of steps.
+    torch.manual_seed(8)
+    w0, g = torch.randn(1000, device="cuda"), torch.randn(1000, device="cuda")
+    ref = optim.AdamW([w0.clone()], state_bits=8, max_grad_norm=1.0)
+    opt = optim.AdamW([w0.clone()], state_bits=8, max_grad_norm=1.0)
+    fresh = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state_dict().items()}
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step([g])
+    for _ in range(2):
+        graph.replay()
+        opt.step([g])
+    for _ in range(4):
+        ref.step([g])
+    assert torch.equal(opt.params[0], ref.params[0]) and opt.state["clocks"][0, 0] == 4
+    opt.load_state_dict(fresh)
+    opt.params[0].copy_(w0)
+    for _ in range(4):
+        graph.replay()
+    assert torch.equal(opt.params[0], ref.params[0])
+
+
+def test_c_entries_refuse_bad_rows():
+    import ctypes
+
+    from diffrast import _lib
+    L, c = _lib.lib(), _lib.ctx_for(0)
+    x = torch.zeros(600, device="cuda")
+    k = torch.zeros(4, dtype=torch.float64, device="cuda")
+    ticket = torch.zeros(1, dtype=torch.int32, device="cuda")
+    work = torch.zeros(4096, dtype=torch.float64, device="cuda")
+    p = x.data_ptr()
+    good = dict(param=p, grad=p + 1024, master=0, m=p + 1600, v=p + 1800, m_scale=p + 2000, v_scale=p + 2100,
+                clock=k.data_ptr(), n=8, lr_ratio=1.0, weight_decay=0.0, seed=0, param_type=0, grad_type=0)
+
+    def step(bits=8, lr=0.0, b1=0.9, eps=1e-8, top=0.0, norm=p + 2200, wk=work.data_ptr(), tick=ticket.data_ptr(), **kw):
+        row = np.zeros(1, optim._ADAMW_ROW)
+        for name, v in {**good, **kw}.items():
+            row[name] = v
+        return L.dr_adamw_step(c, row.ctypes.data, 1, lr, None, b1, 0.999, eps, bits, top, norm, wk, tick)
+
+    assert step() == _lib.DR_OK
+    for kw in (dict(bits=16), dict(lr=-1.0), dict(lr=math.nan), dict(b1=1.0), dict(eps=0.0), dict(eps=1e-40),
+               dict(top=-1.0), dict(top=math.nan), dict(top=1.0, norm=None), dict(top=1.0, wk=None), dict(tick=None),
+               dict(n=-1), dict(n=1 << 62), dict(param=0), dict(grad=0), dict(m=0), dict(clock=0), dict(m_scale=0),
+               dict(param_type=3), dict(grad_type=-1), dict(param_type=1, grad_type=2), dict(master=p),
+               dict(param=p + 2), dict(clock=k.data_ptr() + 4), dict(lr_ratio=-1.0), dict(weight_decay=math.inf)):
+        assert step(**kw) == _lib.DR_EINVAL, kw
+        assert b"adamw" in L.dr_last_error(c)
+
+    def norm(fn, *extra, **kw):
+        row = np.zeros(1, optim._GRAD_ROW)
+        for name, v in {**dict(data=p, n=8, type=0), **kw}.items():
+            row[name] = v
+        return fn(c, row.ctypes.data, 1, *extra, p + 2200, work.data_ptr())
+
+    for fn, extra in ((L.dr_grad_norm, ()), (L.dr_clip_grad_norm, (1.0,))):
+        assert norm(fn, *extra) == _lib.DR_OK
+        for kw in (dict(data=0), dict(n=-1), dict(n=1 << 62), dict(type=5), dict(data=p + 1)):
+            assert norm(fn, *extra, **kw) == _lib.DR_EINVAL, kw
+    for top in (0.0, -1.0, math.nan, math.inf):
+        assert norm(L.dr_clip_grad_norm, top) == _lib.DR_EINVAL
+    assert L.dr_grad_norm(c, None, 1, p, work.data_ptr()) == _lib.DR_EINVAL
+    assert L.dr_grad_norm(c, None, 0, None, work.data_ptr()) == _lib.DR_EINVAL
+    assert L.dr_grad_norm(c, None, -1, p, work.data_ptr()) == _lib.DR_EINVAL
+    torch.cuda.synchronize()
+    assert ctypes.sizeof(ctypes.c_void_p) == 8 and bool((x[:256] == 0).all())
