@@ -91,6 +91,11 @@ __device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const Adam
 constexpr int kStateBlock = 256;
 static_assert(kStateBlock == 32 * kOptVec && kOptChunk % kStateBlock == 0, "one block of states to a warp");
 
+// An 8-bit step's chunk holds kBlocks8 blocks of states for each warp, one in each
+// part of kOptChunk elements.
+constexpr int kBlocks8 = 2;
+constexpr int kChunk8 = kOptChunk * kBlocks8;
+
 // A chunk: its tensor's factors, and where it begins.
 struct AdamSlot {
   AdamFactors f;
@@ -114,7 +119,8 @@ __device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, A
   if (c >= tab.chunks) return;
   const int i = tensor_of(tab.first, tab.count, c);
   const AdamEntry& e = tab.t[i];
-  const int64_t at = (int64_t)(c - tab.first[i]) * kOptChunk;
+  constexpr int kChunk = BITS == 32 ? kOptChunk : kChunk8;
+  const int64_t at = (int64_t)(c - tab.first[i]) * kChunk;
   AdamFactors f;
   if (before && before->tensor == i) f = before->f;
   else f = factors_of(e, tab.h);
@@ -132,7 +138,7 @@ __device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, A
     slot.m_scale = e.m_scale + at / kStateBlock;
     slot.v_scale = e.v_scale + at / kStateBlock;
   }
-  slot.valid = (int)min((int64_t)kOptChunk, e.n - at);
+  slot.valid = (int)min((int64_t)kChunk, e.n - at);
   slot.aligned = e.aligned;
 }
 
@@ -316,8 +322,8 @@ __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c
 
 constexpr uint32_t kGolden = 0x9E3779B9u;
 
-// One thread's elements of a chunk as they lie in memory.  W: the type of the
-// weights that are read, the master's where there are some.
+// One thread's elements of a block of states as they lie in memory.  W: the type
+// of the weights that are read, the master's where there are some.
 template <typename W, typename G>
 struct Fetched {
   Words<W> w;
@@ -327,118 +333,132 @@ struct Fetched {
 };
 
 template <typename W, typename G>
-__device__ __forceinline__ void fetch(const AdamSlot& e, Fetched<W, G>& x) {
-  const unsigned at = threadIdx.x * kOptVec;
+__device__ __forceinline__ void fetch(const AdamSlot& e, int part, Fetched<W, G>& x) {
+  const unsigned at = part * kOptChunk + threadIdx.x * kOptVec, block = part * kOptWarps + threadIdx.x / 32;
   x.w = load_words((const W*)e.weights + at);
   x.g = load_words((const G*)e.grad + at);
   x.m = *reinterpret_cast<const uint2*>((const uint8_t*)e.m + at);
   x.r = *reinterpret_cast<const uint2*>((const uint8_t*)e.v + at);
-  x.m_scale = e.m_scale[threadIdx.x / 32];
-  x.r_scale = e.v_scale[threadIdx.x / 32];
+  x.m_scale = e.m_scale[block];
+  x.r_scale = e.v_scale[block];
 }
 
-// One thread's elements of a chunk, fetched before where WHOLE.  All lanes of a
-// warp, which hold one block of states, come here with the same WHOLE.
-template <bool WHOLE, typename P, typename G, bool MASTER, typename F>
-__device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float eps, float coef, const F& in) {
-  const unsigned at = threadIdx.x * kOptVec;
+// NB blocks of states of a chunk, from part `first` on, one thread's elements of
+// each; fetched before where WHOLE.  All lanes of a warp, which hold one block
+// of each part, come here with the same WHOLE.
+template <bool WHOLE, int NB, typename P, typename G, bool MASTER, typename F>
+__device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float eps, float coef, const F* in,
+                                        int first) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  if (!WHOLE && e.valid <= warp * kStateBlock) return;  // no lane of the warp has elements
-  const int valid = WHOLE ? kOptVec : max(0, min(kOptVec, e.valid - (int)at));
-  P* p = (P*)e.param + at;
-  float* w = (float*)e.weights + at;
-  uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
-  float xp[kOptVec], xg[kOptVec], xm[kOptVec], xr[kOptVec];
-  uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
-  float m_scale, r_scale;
-  if (WHOLE) {
-    widen_words(in.w, xp);
-    widen_words(in.g, xg);
-    cm = in.m;
-    cr = in.r;
-    m_scale = in.m_scale;
-    r_scale = in.r_scale;
-  } else {
-    if (MASTER) load_some(w, valid, xp);
-    else load_some(p, valid, xp);
-    load_some((const G*)e.grad + at, valid, xg);
-#pragma unroll
-    for (int i = 0; i < kOptVec; ++i) {
-      if (i < valid) {
-        (i < 4 ? cm.x : cm.y) |= (uint32_t)m[i] << (8 * (i & 3));
-        (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
-      }
-    }
-    m_scale = e.m_scale[warp];
-    r_scale = e.v_scale[warp];
-  }
-  codes_to_float(cm, xm);
-  codes_to_float(cr, xr);
-  const Two sm = both(m_scale), sr = both(r_scale), kc = both(coef);
+  float xm[NB][kOptVec], xr[NB][kOptVec];
+  float m_top[NB], r_top[NB];
+  const Two kc = both(coef);
   const Two kb1 = both(b.b1), kg1 = both(b.one_m_b1), nb2 = both(-b.b2), ng2 = both(-b.one_m_b2);
   // A sum of two products is a fused operation with a 1 that the compiler does
   // not know: it would make a packed product and sum one, with one rounding.
   const Two one = both(b.one);
   const Two ki = both(-e.f.inv_sqrt), ke = both(eps), ks = both(-e.f.step), kd = both(e.f.decay);
-  float m_top = 0.0f, r_top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kOptVec; i += 2) {
-    const Two gi = two(xg[i], xg[i + 1]) * kc;
-    const Two mi = fma2(two(xm[i], xm[i + 1]) * sm * kb1, one, gi * kg1);
-    const Two r = two(xr[i], xr[i + 1]) * sr;
-    const Two nr = neg_sqrt(fma2(r * r * nb2, one, gi * gi * ng2));  // -v, and -sqrt(v) from here on
-    const float2 d = apart(fma2(nr, ki, ke));
-    const float2 np = apart(fma2(mi * ks, two(rcp_fast(d.x), rcp_fast(d.y)), two(xp[i], xp[i + 1]) * kd));
-    const float2 m2 = apart(mi), r2 = apart(nr);
-    xp[i] = np.x;
-    xp[i + 1] = np.y;
-    // Behind the tensor's end there is nothing: a block of NaN must not reach its scale from there.
-    xm[i] = WHOLE || i < valid ? m2.x : 0.0f;
-    xm[i + 1] = WHOLE || i + 1 < valid ? m2.y : 0.0f;
-    xr[i] = WHOLE || i < valid ? r2.x : 0.0f;
-    xr[i + 1] = WHOLE || i + 1 < valid ? r2.y : 0.0f;
-    m_top = max_nan(m_top, fabsf(xm[i]), fabsf(xm[i + 1]));
-    r_top = max_nan(r_top, fabsf(xr[i]), fabsf(xr[i + 1]));
-  }
-  if (WHOLE) {
-    if (MASTER) store_vec(w, xp);
-    store_vec(p, xp);
-  } else {
-    if (MASTER) store_some(w, valid, xp);
-    store_some(p, valid, xp);
-  }
-  float2 scale, inv;
-  scales_of(m_top, r_top, scale, inv);
-  const uint32_t key = mix(e.f.key + e.block + warp) + (uint32_t)lane * (kOptVec / 2 * kGolden);
-  const Two im = both(inv.x), ir = both(-inv.y), grid = both(0x1p-120f);
-  uint32_t code[kOptVec];
+  for (int n = 0; n < NB; ++n) {
+    const unsigned at = (first + n) * kOptChunk + threadIdx.x * kOptVec;
+    const int valid = WHOLE ? kOptVec : max(0, min(kOptVec, e.valid - (int)at));
+    P* p = (P*)e.param + at;
+    float* w = (float*)e.weights + at;
+    float xp[kOptVec], xg[kOptVec];
+    uint2 cm = make_uint2(0, 0), cr = make_uint2(0, 0);
+    float m_scale, r_scale;
+    if (WHOLE) {
+      widen_words(in[n].w, xp);
+      widen_words(in[n].g, xg);
+      cm = in[n].m;
+      cr = in[n].r;
+      m_scale = in[n].m_scale;
+      r_scale = in[n].r_scale;
+    } else {
+      const uint8_t *m = (const uint8_t*)e.m + at, *v = (const uint8_t*)e.v + at;
+      if (MASTER) load_some(w, valid, xp);
+      else load_some(p, valid, xp);
+      load_some((const G*)e.grad + at, valid, xg);
 #pragma unroll
-  for (int i = 0; i < kOptVec; i += 2) {
-    const float2 qm = apart(two(xm[i], xm[i + 1]) * im);
-    const float2 qr = apart(two(xr[i], xr[i + 1]) * ir * grid);
-    const uint32_t word = mix(key + i / 2 * kGolden);
-    code[i] = round_stochastic<0>(qr.x, xr[i], word);
-    code[i + 1] = round_stochastic<1>(qr.y, xr[i + 1], word);
-    xm[i] = qm.x;
-    xm[i + 1] = qm.y;
-  }
-  cm = float_to_codes(xm);
-  cr = make_uint2(top_bytes(code[0], code[1], code[2], code[3]), top_bytes(code[4], code[5], code[6], code[7]));
-  if (WHOLE) {
-    *reinterpret_cast<uint2*>(m) = cm;
-    *reinterpret_cast<uint2*>(v) = cr;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kOptVec; ++i) {
-      if (i < valid) {
-        m[i] = (uint8_t)((i < 4 ? cm.x : cm.y) >> (8 * (i & 3)));
-        v[i] = (uint8_t)((i < 4 ? cr.x : cr.y) >> (8 * (i & 3)));
+      for (int i = 0; i < kOptVec; ++i) {
+        if (i < valid) {
+          (i < 4 ? cm.x : cm.y) |= (uint32_t)m[i] << (8 * (i & 3));
+          (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
+        }
       }
+      m_scale = e.m_scale[(first + n) * kOptWarps + warp];
+      r_scale = e.v_scale[(first + n) * kOptWarps + warp];
+    }
+    codes_to_float(cm, xm[n]);
+    codes_to_float(cr, xr[n]);
+    const Two sm = both(m_scale), sr = both(r_scale);
+    m_top[n] = r_top[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kOptVec; i += 2) {
+      const Two gi = two(xg[i], xg[i + 1]) * kc;
+      const Two mi = fma2(two(xm[n][i], xm[n][i + 1]) * sm * kb1, one, gi * kg1);
+      const Two r = two(xr[n][i], xr[n][i + 1]) * sr;
+      const Two nr = neg_sqrt(fma2(r * r * nb2, one, gi * gi * ng2));  // -v, and -sqrt(v) from here on
+      const float2 d = apart(fma2(nr, ki, ke));
+      const float2 np = apart(fma2(mi * ks, two(rcp_fast(d.x), rcp_fast(d.y)), two(xp[i], xp[i + 1]) * kd));
+      const float2 m2 = apart(mi), r2 = apart(nr);
+      xp[i] = np.x;
+      xp[i + 1] = np.y;
+      // Behind the tensor's end there is nothing: a block of NaN must not reach its scale from there.
+      xm[n][i] = WHOLE || i < valid ? m2.x : 0.0f;
+      xm[n][i + 1] = WHOLE || i + 1 < valid ? m2.y : 0.0f;
+      xr[n][i] = WHOLE || i < valid ? r2.x : 0.0f;
+      xr[n][i + 1] = WHOLE || i + 1 < valid ? r2.y : 0.0f;
+      m_top[n] = max_nan(m_top[n], fabsf(xm[n][i]), fabsf(xm[n][i + 1]));
+      r_top[n] = max_nan(r_top[n], fabsf(xr[n][i]), fabsf(xr[n][i + 1]));
+    }
+    if (WHOLE) {
+      if (MASTER) store_vec(w, xp);
+      store_vec(p, xp);
+    } else {
+      if (MASTER) store_some(w, valid, xp);
+      store_some(p, valid, xp);
     }
   }
-  if (lane == 0) {
-    e.m_scale[warp] = scale.x;
-    e.v_scale[warp] = scale.y;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const unsigned at = (first + n) * kOptChunk + threadIdx.x * kOptVec, block = (first + n) * kOptWarps + warp;
+    uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
+    float2 scale, inv;
+    scales_of(m_top[n], r_top[n], scale, inv);
+    const uint32_t key = mix(e.f.key + e.block + block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
+    const Two im = both(inv.x), ir = both(-inv.y), grid = both(0x1p-120f);
+    uint32_t code[kOptVec];
+#pragma unroll
+    for (int i = 0; i < kOptVec; i += 2) {
+      const float2 qm = apart(two(xm[n][i], xm[n][i + 1]) * im);
+      const float2 qr = apart(two(xr[n][i], xr[n][i + 1]) * ir * grid);
+      const uint32_t word = mix(key + i / 2 * kGolden);
+      code[i] = round_stochastic<0>(qr.x, xr[n][i], word);
+      code[i + 1] = round_stochastic<1>(qr.y, xr[n][i + 1], word);
+      xm[n][i] = qm.x;
+      xm[n][i + 1] = qm.y;
+    }
+    const uint2 cm = float_to_codes(xm[n]);
+    const uint2 cr =
+        make_uint2(top_bytes(code[0], code[1], code[2], code[3]), top_bytes(code[4], code[5], code[6], code[7]));
+    if (WHOLE) {
+      *reinterpret_cast<uint2*>(m) = cm;
+      *reinterpret_cast<uint2*>(v) = cr;
+    } else {
+      const int valid = max(0, min(kOptVec, e.valid - (int)at));
+#pragma unroll
+      for (int i = 0; i < kOptVec; ++i) {
+        if (i < valid) {
+          m[i] = (uint8_t)((i < 4 ? cm.x : cm.y) >> (8 * (i & 3)));
+          v[i] = (uint8_t)((i < 4 ? cr.x : cr.y) >> (8 * (i & 3)));
+        }
+      }
+    }
+    if (lane == 0) {
+      e.m_scale[block] = scale.x;
+      e.v_scale[block] = scale.y;
+    }
   }
 }
 
@@ -500,11 +520,17 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
 // The arithmetic takes about as long as the memory: a thread's next elements
 // are on their way while it computes.
 template <typename P, typename G, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
+__global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
   using W = typename std::conditional<MASTER, float, P>::type;
   __shared__ AdamSlot s_slots[kRounds][kOptWarps];
   const int warp = threadIdx.x / 32;
-  const auto whole_in = [&](const AdamSlot& e) { return e.aligned && (warp + 1) * kStateBlock <= e.valid; };
+  const auto whole_in = [&](const AdamSlot& e) {
+    return e.aligned && (kBlocks8 - 1) * kOptChunk + (warp + 1) * kStateBlock <= e.valid;
+  };
+  const auto fetch_all = [&](const AdamSlot& e, Fetched<W, G>* x) {
+#pragma unroll
+    for (int n = 0; n < kBlocks8; ++n) fetch(e, n, x[n]);
+  };
   unsigned c = blockIdx.x;
   look_up<P, G, MASTER, 8>(tab, c + warp * gridDim.x, s_slots[0][warp], nullptr);
   float coef;
@@ -512,8 +538,8 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
   __syncthreads();
   const AdamSlot* slot = &s_slots[0][0];
   bool whole = whole_in(*slot);
-  Fetched<W, G> here, next;
-  if (whole) fetch(*slot, here);
+  Fetched<W, G> here[kBlocks8], next[kBlocks8];
+  if (whole) fetch_all(*slot, here);
   for (int round = 0, following = 1, b = 0;;) {
     const AdamSlot* const this_slot = slot;
     const bool this_whole = whole;
@@ -527,15 +553,29 @@ __global__ void __launch_bounds__(kOptThreads, 3) k_adamw8(const __grid_constant
     if (c < tab.chunks) {
       slot = &s_slots[round][b];
       whole = whole_in(*slot);
-      if (whole) fetch(*slot, next);
+      if (whole) fetch_all(*slot, next);
     }
     if (b == 1)  // the next round, whose chunk 0 is kOptWarps - 1 ahead
       look_up<P, G, MASTER, 8>(tab, c + (kOptWarps - 1 + warp) * gridDim.x, s_slots[following][warp],
                                &s_slots[round][warp]);
-    if (this_whole) update8<true, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
-    else update8<false, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here);
+    if (this_whole) {
+      update8<true, kBlocks8, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here, 0);
+    } else {
+#pragma unroll 1
+      for (int n = 0; n < kBlocks8; ++n) {  // a tensor's end, or its pointers are not aligned
+        const int left = this_slot->valid - n * kOptChunk - warp * kStateBlock;
+        if (left >= kStateBlock && this_slot->aligned) {
+          Fetched<W, G> one;
+          fetch(*this_slot, n, one);
+          update8<true, 1, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, &one, n);
+        } else if (left > 0) {
+          update8<false, 1, P, G, MASTER, Fetched<W, G>>(*this_slot, tab.h.betas, tab.h.eps, coef, nullptr, n);
+        }
+      }
+    }
     if (c >= tab.chunks) break;
-    here = next;
+#pragma unroll
+    for (int n = 0; n < kBlocks8; ++n) here[n] = next[n];
   }
   end_step(tab);
 }
@@ -559,7 +599,7 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
       tab.first[tab.count] = (unsigned)chunks;
       tab.t[tab.count++] = {x.param, x.grad, x.master,   x.m,            x.v,    x.m_scale, x.v_scale,
                             x.clock, x.n,    x.lr_ratio, x.weight_decay, x.seed, aligned};
-      chunks += opt_chunks(x.n);
+      chunks += BITS == 32 ? opt_chunks(x.n) : (x.n + kChunk8 - 1) / kChunk8;
     }
     if (tab.count == 0) break;
     tab.chunks = (unsigned)chunks;
