@@ -279,25 +279,16 @@ __device__ __forceinline__ Two neg_sqrt(Two nv) {
   return fma2(fma2(t, t, nv), y * both(0.5f), t);
 }
 
-// Scales of a block's two moments, from each lane's largest magnitudes, and the
-// factors 448 / (largest), rounded to nearest, that take values to codes.
-// Below 2^-100 a block is zero; a value that is not finite makes it NaN.
-__device__ __forceinline__ void scales_of(float m_lane, float r_lane, float2& scale, float2& inv) {
-  // Magnitudes order as their bits do, NaN above infinity.
-  const float2 top = make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m_lane))),
-                                 __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r_lane))));
+// Scale of a block from its largest magnitude, and the factor 448 / (largest),
+// rounded to nearest, that takes values to codes.  Below 2^-100 a block is zero; a
+// value that is not finite makes it NaN.
+__device__ __forceinline__ void scale_of(float top, float& scale, float& inv) {
   // The quotient by a reciprocal and its residual, as for the root; all times 2^-20, for the reciprocal of a large one.
-  const Two t = two(fmaxf(top.x, 0x1p-100f), fmaxf(top.y, 0x1p-100f)) * both(0x1p-20f);
-  const Two k = both(-kMaxCode * 0x1p-20f);
-  const float2 tt = apart(t);
-  const Two y = two(rcp_fast(-tt.x), rcp_fast(-tt.y));
-  const Two q = k * y;
-  inv = apart(fma2(fma2(q, t, k), y, q));
-  // top - top: 0, or NaN for what is not finite
-  scale = make_float2(__fmaf_rn(top.x, 1.0f / kMaxCode, __fsub_rn(top.x, top.x)),
-                      __fmaf_rn(top.y, 1.0f / kMaxCode, __fsub_rn(top.y, top.y)));
-  if (top.x < 0x1p-100f) scale.x = inv.x = 0.0f;
-  if (top.y < 0x1p-100f) scale.y = inv.y = 0.0f;
+  const float t = __fmul_rn(fmaxf(top, 0x1p-100f), 0x1p-20f), k = -kMaxCode * 0x1p-20f;
+  const float y = rcp_fast(-t), q = __fmul_rn(k, y);
+  inv = __fmaf_rn(__fmaf_rn(q, t, k), y, q);
+  scale = __fmaf_rn(top, 1.0f / kMaxCode, __fsub_rn(top, top));  // top - top: 0, or NaN for what is not finite
+  if (top < 0x1p-100f) scale = inv = 0.0f;
 }
 
 // The code of a value, given its negative (or +0) and z = 2^-120 (value / scale):
@@ -420,14 +411,26 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
       store_some(p, valid, xp);
     }
   }
+  // The scales of the 2 NB blocks of moments, each formed in eight lanes.
+  static_assert(2 * NB <= 4, "eight lanes to a block");
+  float top = 0.0f, scale, inv;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    // Magnitudes order as their bits do, NaN above infinity.
+    const float m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m_top[n])));
+    const float r = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r_top[n])));
+    if (lane / 16 == n) top = lane & 8 ? r : m;
+  }
+  scale_of(top, scale, inv);
+  if (lane % 8 == 0 && lane < 16 * NB)
+    ((lane & 8) ? e.v_scale : e.m_scale)[(first + lane / 16) * kOptWarps + warp] = scale;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const unsigned at = (first + n) * kOptChunk + threadIdx.x * kOptVec, block = (first + n) * kOptWarps + warp;
     uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
-    float2 scale, inv;
-    scales_of(m_top[n], r_top[n], scale, inv);
+    const float m_inv = __shfl_sync(0xffffffffu, inv, 16 * n), r_inv = __shfl_sync(0xffffffffu, inv, 16 * n + 8);
     const uint32_t key = mix(e.f.key + e.block + block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
-    const Two im = both(inv.x), ir = both(-inv.y), grid = both(0x1p-120f);
+    const Two im = both(m_inv), ir = both(-r_inv), grid = both(0x1p-120f);
     uint32_t code[kOptVec];
 #pragma unroll
     for (int i = 0; i < kOptVec; i += 2) {
@@ -454,10 +457,6 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
           v[i] = (uint8_t)((i < 4 ? cr.x : cr.y) >> (8 * (i & 3)));
         }
       }
-    }
-    if (lane == 0) {
-      e.m_scale[block] = scale.x;
-      e.v_scale[block] = scale.y;
     }
   }
 }

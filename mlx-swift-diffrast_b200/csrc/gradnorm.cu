@@ -79,7 +79,7 @@ __device__ __forceinline__ void fetch(const GradSlot& e, Fetched& x, double& s) 
   const int bytes = e.type == DR_F32 ? 4 : 2, valid = e.valid - (int)threadIdx.x * kOptVec;
   const char* p = e.data + threadIdx.x * kOptVec * bytes;
   x.type = -1;
-  if (valid >= kOptVec && (uintptr_t)p % (kOptVec * bytes) == 0) {
+  if (valid >= kOptVec && ((uintptr_t)p & (kOptVec * bytes - 1)) == 0) {
     x.type = e.type;
     if (e.type == DR_F32) x.w = load_words((const float*)p);
     else x.w.w[0] = load_words((const __half*)p).w[0];
