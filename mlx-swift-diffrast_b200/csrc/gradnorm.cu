@@ -21,8 +21,10 @@ struct GradEntry {
 };
 
 // A launch carries its list as a parameter, which a captured graph keeps: no
-// table in device memory that a replay would have to find unchanged.  Small
-// lists use a small parameter block.
+// table in device memory that a replay would have to find unchanged.  The block
+// comes in three sizes: the host copies all of it at each launch, and 28 KB of
+// it cost 2 us where 2 KB cost next to nothing (the norm of two small tensors:
+// 13.5 us with the small block, 15.7 with the large one).
 template <int CAP>
 struct GradTable {
   GradEntry t[CAP];
@@ -30,7 +32,7 @@ struct GradTable {
   int count;
   unsigned chunks;
 };
-constexpr int kSmall = 64, kLarge = 1000;
+constexpr int kSmall = 64, kMedium = 250, kLarge = 1000;
 static_assert(sizeof(GradTable<kLarge>) + 64 <= 32764, "kernel parameters");
 
 // Partial sums per launch at most, whatever the device.
@@ -269,8 +271,9 @@ dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* no
 dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts,
                           float* norm) {
   *parts = 0;
-  return count <= kSmall ? launch_parts<kSmall>(ctx, grads, count, work, parts, norm)
-                         : launch_parts<kLarge>(ctx, grads, count, work, parts, norm);
+  return count <= kSmall    ? launch_parts<kSmall>(ctx, grads, count, work, parts, norm)
+         : count <= kMedium ? launch_parts<kMedium>(ctx, grads, count, work, parts, norm)
+                            : launch_parts<kLarge>(ctx, grads, count, work, parts, norm);
 }
 
 }  // namespace dr
@@ -309,8 +312,10 @@ dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count,
   int parts = 0;
   if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, nullptr)) != DR_OK) return st;
   if (parts == 0) return grad_norm_finish(ctx, (const double*)work, 0, norm);  // nothing to scale
-  return count <= kSmall ? launch_scale<kSmall>(ctx, grads, count, (const double*)work, parts, max_norm, norm)
-                         : launch_scale<kLarge>(ctx, grads, count, (const double*)work, parts, max_norm, norm);
+  const double* part = (const double*)work;
+  return count <= kSmall    ? launch_scale<kSmall>(ctx, grads, count, part, parts, max_norm, norm)
+         : count <= kMedium ? launch_scale<kMedium>(ctx, grads, count, part, parts, max_norm, norm)
+                            : launch_scale<kLarge>(ctx, grads, count, part, parts, max_norm, norm);
 }
 
 }  // extern "C"

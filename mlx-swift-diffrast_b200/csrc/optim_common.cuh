@@ -67,15 +67,6 @@ __device__ __forceinline__ void widen_words(const Words<T>& words, float (&x)[kO
   for (int i = 0; i < kOptVec; ++i) x[i] = widen(e[i]);
 }
 
-// The same from shared memory.
-template <typename T>
-__device__ __forceinline__ void shared_vec(const T* p, float (&x)[kOptVec]) {
-  Words<T> words;
-#pragma unroll
-  for (int i = 0; i < Words<T>::kCount; ++i) words.w[i] = reinterpret_cast<const uint4*>(p)[i];
-  widen_words(words, x);
-}
-
 template <typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[kOptVec]) {
   widen_words(load_words(p), x);
@@ -99,6 +90,16 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[kOptVec]) {
 template <typename T>
 __host__ __device__ __forceinline__ bool vector_aligned(const T* p) {
   return (uintptr_t)p % (kOptVec * sizeof(T)) == 0;
+}
+
+// load_words at any address of T's alignment.
+template <typename T>
+__device__ __forceinline__ Words<T> gather_words(const T* p) {
+  Words<T> x;
+  T* e = reinterpret_cast<T*>(x.w);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) e[i] = p[i];
+  return x;
 }
 
 // `valid` (0 .. kOptVec) elements at any address of T's alignment; the others are 0.
