@@ -4,10 +4,17 @@
 //   p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Every operation on elements is a separate IEEE round-to-nearest step in
-// float, so a step is the same bit for bit as an unfused evaluation.  The
-// factors in t are formed in double on the device from each tensor's clock
-// (t, b1^t, b2^t), which the step itself advances: nothing in a captured step
-// is fixed to the t of its capture.
+// float, so moments, states and (32-bit states) parameters are the same bit for
+// bit as an unfused evaluation; with 8-bit states the parameter's quotient is a
+// product with the hardware's reciprocal.  The factors in t are formed in double
+// on the device from each tensor's clock (t, b1^t, b2^t), which the step itself
+// advances: nothing in a captured step is fixed to the t of its capture.
+//
+// 32-bit states are bound by memory: 28 bytes an element in fp32, 1150 us for
+// sixteen 2048^2x4 textures (268 M elements, 7.5 GB), 6.5 TB/s.  8-bit states move
+// 16 (fp32) or 10 bytes (16-bit types) and are bound by issue: 355 instructions
+// for a block of 256 elements, most of them the exact roundings, the root, the
+// random bits and the codes; the same textures in fp16 take 500 us, 5.4 TB/s.
 #include <new>
 #include <type_traits>
 
@@ -227,7 +234,7 @@ __device__ __forceinline__ uint2 float_to_codes(const float (&x)[kOptVec]) {
 }
 
 // Two floats in a register pair: one instruction for both, each rounded as
-// the single one is.
+// the single one is (fp16 textures: 547 us with them, 594 with single ones).
 struct Two {
   uint64_t v;
 };
@@ -504,6 +511,12 @@ __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   if (threadIdx.x == 0) *h.ticket = 0;
 }
 
+// A chunk of 2048 elements at a time, four blocks to a multiprocessor, whose
+// waits hide each other.  More and shorter-lived blocks stream one large list
+// slightly faster (64 to a multiprocessor: 1140 us for the sixteen textures) but
+// start dearly on lists of many tensors (120 bf16 tensors with master weights:
+// 110 us; 127 with 64).  Fetching the next chunk during the arithmetic takes the
+// registers of two of the four blocks (1560 us).
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ AdamTable<CAP> tab) {
   __shared__ AdamSlot s_slots[kRounds][kOptWarps];
@@ -525,7 +538,13 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
 }
 
 // The arithmetic takes about as long as the memory: a thread's next elements
-// are on their way while it computes.
+// are on their way while it computes.  One wave of two blocks to a multiprocessor
+// with two blocks of states to a warp: their instructions interleave and share
+// constants and addresses.  Sixteen textures in fp16: 500 us; with one block of
+// states to a warp and three blocks 547; the same with the next elements on
+// their way through shared memory, by asynchronous or bulk copies, 528 and 667
+// (64 registers, in which the packed constants do not stay); not fetched ahead
+// at all 620 and more.
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
   using W = typename std::conditional<MASTER, float, P>::type;
