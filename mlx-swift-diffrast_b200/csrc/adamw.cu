@@ -92,7 +92,7 @@ __device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const Adam
   AdamFactors f;
   f.decay = (float)(1.0 - lr * e.weight_decay);
   f.step = (float)(lr / (1.0 - b1t));
-  f.inv_sqrt = (float)(1.0 / sqrt(1.0 - b2t));
+  f.inv_sqrt = (float)rsqrt(1.0 - b2t);
   f.key = mix(mix((uint32_t)(long long)t) ^ e.seed);
   return f;
 }
@@ -489,26 +489,23 @@ __device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
 }
 
 // The last block to come here has every other block's reads of the clocks
-// behind it: it advances them, and leaves the ticket as it found it.
+// behind it (their values were used before its ticket was drawn, so no fence is
+// needed): it advances them, and leaves the ticket as it found it.
 template <int CAP>
 __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   const AdamHyper& h = tab.h;
   __shared__ bool s_last;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicAdd(h.ticket, 1u) == gridDim.x - 1;
-  }
+  if (threadIdx.x == 0) s_last = gridDim.x == 1 || atomicAdd(h.ticket, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
   for (int i = threadIdx.x; i < tab.count; i += kOptThreads) {
     double* k = tab.t[i].clock;
     k[0] += 1.0;
     k[1] *= h.beta1;
     k[2] *= h.beta2;
   }
-  if (threadIdx.x == 0) *h.ticket = 0;
+  if (threadIdx.x == 0 && gridDim.x > 1) *h.ticket = 0;
 }
 
 // A chunk of 2048 elements at a time, four blocks to a multiprocessor, whose

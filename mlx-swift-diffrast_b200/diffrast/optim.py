@@ -7,6 +7,7 @@ in fp32, bf16 or fp16, AdamW's states in 32 or in 8 bits.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import Optional, Sequence, Union
@@ -130,41 +131,44 @@ def _written(ts) -> None:
         torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
 
 
-def _context(index: int):
-    """The context of a device, on torch's current stream there."""
+@functools.lru_cache(maxsize=None)
+def _context(index: int) -> int:
+    """The address of a device's context; binds the library's functions at the first call."""
     c = L.ctx_for(index)
-    L.lib().dr_ctx_set_stream(c, torch._C._cuda_getCurrentRawStream(index))
-    return c
+    lib = L.lib()
+    _rows.bind(*(ctypes.cast(f, ctypes.c_void_p).value
+                 for f in (lib.dr_ctx_set_stream, lib.dr_grad_norm, lib.dr_clip_grad_norm, lib.dr_adamw_step)))
+    return c.value
 
 
 @functools.lru_cache(maxsize=256)
 def _work_len(index: int, count: int) -> int:
-    return int(L.lib().dr_grad_norm_work_bytes(L.ctx_for(index), count)) // 8
+    return int(L.lib().dr_grad_norm_work_bytes(_context(index), count)) // 8
 
 
 def _norm_work(index: int, count: int) -> torch.Tensor:
     return torch.empty(_work_len(index, count), dtype=torch.float64, device=_CUDA[index])
 
 
-def _norm_call(fn, ts, what: str, apart: bool, dense, *args) -> torch.Tensor:
-    """fn (dr_grad_norm or dr_clip_grad_norm) on the list `ts`; the norm.  dense: what the tensors become that are not
-    contiguous."""
-    found = _rows.grads(ts, apart)
+def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
+    """The norm of the list `ts`; with max_norm > 0 the list is clipped by it.  dense: what the tensors become that are
+    not contiguous."""
+    found = _rows.grads(ts, max_norm > 0.0)
     if found is None:
         ts = [t if t.is_contiguous() else dense(t) for t in _check_list(ts, what)]
-        if apart:
+        if max_norm > 0.0:
             _check_apart(ts, what)
         found = ts[0].get_device(), _grad_table(ts).tobytes()
     index, rows = found
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            return _norm_call(fn, ts, what, apart, dense, *args)
+            return _norm_call(ts, what, max_norm, dense)
     c = _context(index)
     # From torch's allocator at each call: both belong to the stream (or to the
     # graph being captured) and to no other call.
     norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
     work = _norm_work(index, len(ts))
-    status = fn(c, rows, len(ts), *args, norm.data_ptr(), work.data_ptr())
+    status = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), work.data_ptr())
     if status:
         L.check(status, c, what)
     return norm
@@ -176,8 +180,7 @@ def grad_norm(grads) -> torch.Tensor:
     their device, the same from run to run.  Squares are summed in 64 bits, so
     the norm is finite wherever float32 holds it."""
     ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    return _norm_call(L.lib().dr_grad_norm, ts, "grad_norm", False,
-                      lambda t: t if _dense(t) else t.detach().contiguous())
+    return _norm_call(ts, "grad_norm", 0.0, lambda t: t if _dense(t) else t.detach().contiguous())
 
 
 def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
@@ -195,7 +198,7 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
             raise ValueError("clip_grad_norm_: tensors must fill their memory (they are scaled in place)")
         return t
 
-    norm = _norm_call(L.lib().dr_clip_grad_norm, ts, "clip_grad_norm_", True, dense, max_norm)
+    norm = _norm_call(ts, "clip_grad_norm_", max_norm, dense)
     _written(ts)
     return norm
 
@@ -306,8 +309,7 @@ class AdamW:
         # the parameters must still be there.
         self._held = [p.detach() for p in self.params]
         self._addresses = tab["param"][:] = [p.data_ptr() for p in self.params]
-        self._at = tab.ctypes.data
-        self._index, self._device = dev.index, dev
+        self._index, self._device, self._context = dev.index, dev, _context(dev.index)
         with torch.cuda.device(dev):
             # A step's own: steps of one optimizer never run side by side.
             self._work = _norm_work(dev.index, count)
@@ -377,8 +379,13 @@ class AdamW:
         lr, lr_dev, top = self._step_args()
         if lr_dev is not None and lr_dev.get_device() != self._index:
             raise ValueError("AdamW: a learning_rate tensor must be on the parameters' device")
-        at, rows = ps, self._at
-        if _rows.step(ps, grads, self._tab, self._index) != 0:
+        norm = torch.empty((), dtype=torch.float32, device=self._device) if top else None
+        args = (self._index, self._context, lr, None if lr_dev is None else lr_dev.data_ptr(), self.beta1, self.beta2,
+                self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(), self._work_at,
+                self._ticket_at)
+        at = ps
+        status = _rows.step(ps, grads, self._tab, *args)
+        if status < 0:
             gs = [p.grad for p in ps] if grads is None else list(grads)
             if len(gs) != len(ps):
                 raise ValueError(f"AdamW: {len(ps)} gradients expected (got {len(gs)})")
@@ -389,15 +396,9 @@ class AdamW:
             at, gs, table = [ps[i] for i in keep], [gs[i] for i in keep], self._tab[keep]
             table["grad"] = [g.data_ptr() for g in gs]
             table["grad_type"] = [_TYPES[g.dtype] for g in gs]
-            rows = table.tobytes()
-        c = _context(self._index)
-        norm = torch.empty((), dtype=torch.float32, device=self._device) if top else None
-        status = L.lib().dr_adamw_step(
-            c, rows, len(at), lr, None if lr_dev is None else lr_dev.data_ptr(),
-            self.beta1, self.beta2, self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(),
-            self._work_at, self._ticket_at)
+            status = _rows.step(None, None, table.tobytes(), *args)
         if status:
-            L.check(status, c, "AdamW")
+            L.check(status, self._context, "AdamW")
         _written(at)
         return norm
 

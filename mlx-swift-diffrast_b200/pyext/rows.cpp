@@ -4,8 +4,8 @@
 // A step over many tensors asks each for its address, sizes, strides, type and
 // device.  From Python that is 0.8 us a tensor, more than the GPU's work on
 // small ones; here it is 0.1 us.  Tensors are read through the DLPack exchange
-// functions that torch.Tensor publishes, so nothing of torch is linked.  Every
-// function answers only for lists that are simple (dense, contiguous, of known
+// functions that torch.Tensor publishes, so nothing of torch is linked.  The look
+// at the lists answers only for lists that are simple (dense, contiguous, of known
 // types, on one CUDA device) and otherwise returns None or -1, upon which the
 // Python side looks at the tensors one by one and raises or copies.
 #define PY_SSIZE_T_CLEAN
@@ -132,20 +132,92 @@ PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return found;
 }
 
-// step(params, grads or None, table, device) -> 0, or -1: looks each parameter
-// (its address is its row's, see below) and gradient over and fills the rows'
-// grad and grad_type.  grads None: the parameters' .grad.
+// The C ABI's functions, from the binding that has loaded the library: called
+// from here they cost 2 us less than through ctypes.
+decltype(&dr_ctx_set_stream) set_stream = nullptr;
+decltype(&dr_grad_norm) grad_norm = nullptr;
+decltype(&dr_clip_grad_norm) clip_grad_norm = nullptr;
+decltype(&dr_adamw_step) adamw_step = nullptr;
+
+// bind(dr_ctx_set_stream, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step): their addresses.
+PyObject* bind(PyObject*, PyObject* args) {
+  unsigned long long a, b, c, d;
+  if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return nullptr;
+  set_stream = reinterpret_cast<decltype(set_stream)>(a);
+  grad_norm = reinterpret_cast<decltype(grad_norm)>(b);
+  clip_grad_norm = reinterpret_cast<decltype(clip_grad_norm)>(c);
+  adamw_step = reinterpret_cast<decltype(adamw_step)>(d);
+  Py_RETURN_NONE;
+}
+
+template <typename T>
+T* pointer(PyObject* o) {
+  return o == Py_None ? nullptr : static_cast<T*>(PyLong_AsVoidPtr(o));
+}
+
+// Puts the context on torch's current stream of the device; false with an exception set.
+bool on_current_stream(dr_ctx* ctx, long device) {
+  void* stream = nullptr;
+  if (api->current_work_stream(kCuda, (int32_t)device, &stream) != 0) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "no current stream");
+    return false;
+  }
+  set_stream(ctx, stream);
+  return true;
+}
+
+// norm(ctx, device, rows, max_norm, norm, work) -> status: dr_grad_norm, or with max_norm > 0 dr_clip_grad_norm,
+// of the rows (bytes) that grads() or the Python side made.
+PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6 || !PyBytes_Check(args[2]) || !set_stream) {
+    PyErr_SetString(PyExc_TypeError, "norm(ctx, device, rows, max_norm, norm, work)");
+    return nullptr;
+  }
+  auto* ctx = pointer<dr_ctx>(args[0]);
+  const long device = PyLong_AsLong(args[1]);
+  const auto* rows = reinterpret_cast<const dr_grad_tensor*>(PyBytes_AS_STRING(args[2]));
+  const int count = (int)(PyBytes_GET_SIZE(args[2]) / (Py_ssize_t)sizeof(dr_grad_tensor));
+  const double max_norm = PyFloat_AsDouble(args[3]);
+  auto* out = pointer<float>(args[4]);
+  auto* work = pointer<void>(args[5]);
+  if (PyErr_Occurred() || !on_current_stream(ctx, device)) return nullptr;
+  dr_status st;
+  Py_BEGIN_ALLOW_THREADS
+  st = max_norm > 0.0 ? clip_grad_norm(ctx, rows, count, max_norm, out, work) : grad_norm(ctx, rows, count, out, work);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
+// step(params, grads, table, device, ctx, lr, lr_device, beta1, beta2, eps, bits, max_norm, norm, work, ticket)
+// -> status, or -1.  Looks each parameter (its address is its row's, see below) and gradient over, fills the rows'
+// grad and grad_type and calls dr_adamw_step.  grads None: the parameters' .grad.  params None: the rows (bytes)
+// are filled, and -1 does not come back.
 PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  Py_ssize_t n = 0, ng = 0;
-  PyObject** ps = nargs == 4 ? items(args[0], n) : nullptr;
-  PyObject** gs = nargs == 4 && args[1] != Py_None ? items(args[1], ng) : nullptr;
-  if (!ps || (args[1] != Py_None && (!gs || ng != n))) return PyLong_FromLong(-1);
-  Py_buffer table;
-  if (PyObject_GetBuffer(args[2], &table, PyBUF_WRITABLE) != 0) return nullptr;
+  if (nargs != 15 || !set_stream) {
+    PyErr_SetString(PyExc_TypeError, "step: 15 arguments");
+    return nullptr;
+  }
+  auto* ctx = pointer<dr_ctx>(args[4]);
   const long device = PyLong_AsLong(args[3]);
+  const double lr = PyFloat_AsDouble(args[5]), beta1 = PyFloat_AsDouble(args[7]), beta2 = PyFloat_AsDouble(args[8]);
+  const double eps = PyFloat_AsDouble(args[9]), max_norm = PyFloat_AsDouble(args[11]);
+  const int bits = (int)PyLong_AsLong(args[10]);
+  auto* lr_device = pointer<const float>(args[6]);
+  auto* out = pointer<float>(args[12]);
+  auto* work = pointer<void>(args[13]);
+  auto* ticket = pointer<uint32_t>(args[14]);
+  if (PyErr_Occurred()) return nullptr;
+  Py_buffer table;
+  Py_ssize_t n = 0, ng = 0;
+  const bool ready = args[0] == Py_None;
+  PyObject** ps = ready ? nullptr : items(args[0], n);
+  PyObject** gs = args[1] != Py_None ? items(args[1], ng) : nullptr;
+  if (!ready && (!ps || (args[1] != Py_None && (!gs || ng != n)))) return PyLong_FromLong(-1);
+  if (PyObject_GetBuffer(args[2], &table, ready ? PyBUF_SIMPLE : PyBUF_WRITABLE) != 0) return nullptr;
+  if (ready) n = table.len / (Py_ssize_t)sizeof(dr_adamw_tensor);
   bool fine = table.len >= n * (Py_ssize_t)sizeof(dr_adamw_tensor);
   auto* rows = static_cast<dr_adamw_tensor*>(table.buf);
-  for (Py_ssize_t i = 0; fine && i < n; ++i) {
+  for (Py_ssize_t i = 0; fine && !ready && i < n; ++i) {
     Seen p, g;
     // The caller's memory is held since the optimizer was made, so nothing
     // else can have come to its address.
@@ -167,13 +239,25 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (!gs) Py_DECREF(grad);  // the parameter holds it
   }
+  long st = -1;
+  bool error = false;
+  if (fine) {
+    error = !on_current_stream(ctx, device);
+    if (!error) {
+      Py_BEGIN_ALLOW_THREADS
+      st = adamw_step(ctx, rows, (int)n, lr, lr_device, beta1, beta2, eps, bits, max_norm, out, work, ticket);
+      Py_END_ALLOW_THREADS
+    }
+  }
   PyBuffer_Release(&table);
-  return PyLong_FromLong(fine ? 0 : -1);
+  return error ? nullptr : PyLong_FromLong(st);
 }
 
 PyMethodDef methods[] = {
     {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows) or None"},
-    {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads or None, table, device -> 0 or -1"},
+    {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
+    {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> status"},
+    {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads, table, ... -> status or -1"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", "Tensors to the C ABI's rows.", -1, methods,
@@ -190,7 +274,7 @@ PyMODINIT_FUNC PyInit__rows() {
   api = static_cast<const DLPackExchangeAPI*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api"));
   Py_DECREF(capsule);
   if (!api) return nullptr;
-  if (api->major != 1 || !api->dltensor_from_py_object_no_sync) {
+  if (api->major != 1 || !api->dltensor_from_py_object_no_sync || !api->current_work_stream) {
     PyErr_SetString(PyExc_ImportError, "torch's DLPack exchange table is of another version");
     return nullptr;
   }
