@@ -14,7 +14,7 @@
 // sixteen 2048^2x4 textures (268 M elements, 7.5 GB), 6.5 TB/s.  8-bit states move
 // 16 (fp32) or 10 bytes (16-bit types) and are bound by issue: 355 instructions
 // for a block of 256 elements, most of them the exact roundings, the root, the
-// random bits and the codes; the same textures in fp16 take 500 us, 5.4 TB/s.
+// random bits and the codes; the same textures in fp16 take 475 us, 5.7 TB/s.
 #include <new>
 #include <type_traits>
 
@@ -99,12 +99,13 @@ __device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const Adam
 
 // 8-bit states: a warp holds a block of 256 elements, eight to a lane.
 constexpr int kStateBlock = 256;
-static_assert(kStateBlock == 32 * kOptVec && kOptChunk % kStateBlock == 0, "one block of states to a warp");
+static_assert(kStateBlock == 32 * kOptVec, "one block of states to a warp");
 
-// An 8-bit step's chunk holds kBlocks8 blocks of states for each warp, one in each
-// part of kOptChunk elements.
+// An 8-bit step's block has 16 warps, and its chunk kBlocks8 blocks of states for
+// each, one in each part of kPart8 elements.
+constexpr int kThreads8 = 512, kWarps8 = kThreads8 / 32;
 constexpr int kBlocks8 = 2;
-constexpr int kChunk8 = kOptChunk * kBlocks8;
+constexpr int kPart8 = kThreads8 * kOptVec, kChunk8 = kPart8 * kBlocks8;
 
 // A chunk: its tensor's factors, and where it begins.
 struct AdamSlot {
@@ -335,7 +336,7 @@ struct Fetched {
 
 template <typename W, typename G>
 __device__ __forceinline__ void fetch(const AdamSlot& e, int part, Fetched<W, G>& x) {
-  const unsigned at = part * kOptChunk + threadIdx.x * kOptVec, block = part * kOptWarps + threadIdx.x / 32;
+  const unsigned at = part * kPart8 + threadIdx.x * kOptVec, block = part * kWarps8 + threadIdx.x / 32;
   if (e.aligned & kVectors) {
     x.w = load_words((const W*)e.weights + at);
     x.g = load_words((const G*)e.grad + at);
@@ -366,7 +367,7 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
   const Two ki = both(-e.f.inv_sqrt), ke = both(eps), ks = both(-e.f.step), kd = both(e.f.decay);
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const unsigned at = (first + n) * kOptChunk + threadIdx.x * kOptVec;
+    const unsigned at = (first + n) * kPart8 + threadIdx.x * kOptVec;
     const int valid = WHOLE ? kOptVec : max(0, min(kOptVec, e.valid - (int)at));
     P* p = (P*)e.param + at;
     float* w = (float*)e.weights + at;
@@ -392,8 +393,8 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
           (i < 4 ? cr.x : cr.y) |= (uint32_t)v[i] << (8 * (i & 3));
         }
       }
-      m_scale = e.m_scale[(first + n) * kOptWarps + warp];
-      r_scale = e.v_scale[(first + n) * kOptWarps + warp];
+      m_scale = e.m_scale[(first + n) * kWarps8 + warp];
+      r_scale = e.v_scale[(first + n) * kWarps8 + warp];
     }
     codes_to_float(cm, xm[n]);
     codes_to_float(cr, xr[n]);
@@ -438,10 +439,10 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
   }
   scale_of(top, scale, inv);
   if (lane % 8 == 0 && lane < 16 * NB)
-    ((lane & 8) ? e.v_scale : e.m_scale)[(first + lane / 16) * kOptWarps + warp] = scale;
+    ((lane & 8) ? e.v_scale : e.m_scale)[(first + lane / 16) * kWarps8 + warp] = scale;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const unsigned at = (first + n) * kOptChunk + threadIdx.x * kOptVec, block = (first + n) * kOptWarps + warp;
+    const unsigned at = (first + n) * kPart8 + threadIdx.x * kOptVec, block = (first + n) * kWarps8 + warp;
     uint8_t *m = (uint8_t*)e.m + at, *v = (uint8_t*)e.v + at;
     const float m_inv = __shfl_sync(0xffffffffu, inv, 16 * n), r_inv = __shfl_sync(0xffffffffu, inv, 16 * n + 8);
     const uint32_t key = mix(e.f.key + e.block + block) + (uint32_t)lane * (kOptVec / 2 * kGolden);
@@ -478,11 +479,12 @@ __device__ __forceinline__ void update8(const AdamSlot& e, const Betas& b, float
 
 // The clipping factor, which every block of a step forms for itself.  False
 // where the step is to change nothing.
+template <int THREADS>
 __device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
   coef = 1.0f;
   if (!h.part) return true;
   after_previous();
-  const double norm = norm_of(h.part, h.parts);
+  const double norm = norm_of<THREADS>(h.part, h.parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
   coef = clip_factor(norm, h.max_norm);
   return isfinite(norm);  // the same in every block
@@ -499,7 +501,7 @@ __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   if (threadIdx.x == 0) s_last = gridDim.x == 1 || atomicAdd(h.ticket, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!s_last) return;
-  for (int i = threadIdx.x; i < tab.count; i += kOptThreads) {
+  for (int i = threadIdx.x; i < tab.count; i += blockDim.x) {
     double* k = tab.t[i].clock;
     k[0] += 1.0;
     k[1] *= h.beta1;
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
   unsigned c = blockIdx.x;
   look_up<P, G, MASTER, 32>(tab, c + warp * gridDim.x, s_slots[0][warp], nullptr);
   float coef;
-  if (!begin_step(tab.h, coef)) return;
+  if (!begin_step<kOptThreads>(tab.h, coef)) return;
   __syncthreads();
   for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
     look_up<P, G, MASTER, 32>(tab, c + (kOptWarps + warp) * gridDim.x,
@@ -535,20 +537,21 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
 }
 
 // The arithmetic takes about as long as the memory: a thread's next elements
-// are on their way while it computes.  One wave of two blocks to a multiprocessor
-// with two blocks of states to a warp: their instructions interleave and share
-// constants and addresses.  Sixteen textures in fp16: 500 us; with one block of
-// states to a warp and three blocks 547; the same with the next elements on
-// their way through shared memory, by asynchronous or bulk copies, 528 and 667
-// (64 registers, in which the packed constants do not stay); not fetched ahead
-// at all 620 and more.
+// are on their way while it computes.  One wave of one block of 16 warps to a
+// multiprocessor, two blocks of states to a warp: their instructions interleave
+// and share constants and addresses.  Sixteen textures in fp16: 475 us on the
+// device (545 in a long run, where the power limit holds the clock down); with
+// two blocks of 8 warps 500 (565), which start 0.3 us faster on small lists; with
+// one block of states to a warp and three blocks 547; the same with the next
+// elements on their way through shared memory, by asynchronous or bulk copies,
+// 528 and 667 (64 registers, in which the packed constants do not stay).
 template <typename P, typename G, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
+__global__ void __launch_bounds__(kThreads8, 1) k_adamw8(const __grid_constant__ AdamTable<CAP> tab) {
   using W = typename std::conditional<MASTER, float, P>::type;
-  __shared__ AdamSlot s_slots[kRounds][kOptWarps];
+  __shared__ AdamSlot s_slots[kRounds][kWarps8];
   const int warp = threadIdx.x / 32;
   const auto whole_in = [&](const AdamSlot& e) {
-    return (e.aligned & kCodes) && (kBlocks8 - 1) * kOptChunk + (warp + 1) * kStateBlock <= e.valid;
+    return (e.aligned & kCodes) && (kBlocks8 - 1) * kPart8 + (warp + 1) * kStateBlock <= e.valid;
   };
   const auto fetch_all = [&](const AdamSlot& e, Fetched<W, G>* x) {
 #pragma unroll
@@ -557,7 +560,7 @@ __global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant
   unsigned c = blockIdx.x;
   look_up<P, G, MASTER, 8>(tab, c + warp * gridDim.x, s_slots[0][warp], nullptr);
   float coef;
-  if (!begin_step(tab.h, coef)) return;
+  if (!begin_step<kThreads8>(tab.h, coef)) return;
   __syncthreads();
   const AdamSlot* slot = &s_slots[0][0];
   bool whole = whole_in(*slot);
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant
     const AdamSlot* const this_slot = slot;
     const bool this_whole = whole;
     c += gridDim.x;
-    if (++b == kOptWarps) {
+    if (++b == kWarps8) {
       b = 0;
       round = following;
       if (++following == kRounds) following = 0;
@@ -578,15 +581,15 @@ __global__ void __launch_bounds__(kOptThreads, 2) k_adamw8(const __grid_constant
       whole = whole_in(*slot);
       if (whole) fetch_all(*slot, next);
     }
-    if (b == 1)  // the next round, whose chunk 0 is kOptWarps - 1 ahead
-      look_up<P, G, MASTER, 8>(tab, c + (kOptWarps - 1 + warp) * gridDim.x, s_slots[following][warp],
+    if (b == 1)  // the next round, whose chunk 0 is kWarps8 - 1 ahead
+      look_up<P, G, MASTER, 8>(tab, c + (kWarps8 - 1 + warp) * gridDim.x, s_slots[following][warp],
                                &s_slots[round][warp]);
     if (this_whole) {
       update8<true, kBlocks8, P, G, MASTER>(*this_slot, tab.h.betas, tab.h.eps, coef, here, 0);
     } else {
 #pragma unroll 1
       for (int n = 0; n < kBlocks8; ++n) {  // a tensor's end, or its pointers are not aligned
-        const int left = this_slot->valid - n * kOptChunk - warp * kStateBlock;
+        const int left = this_slot->valid - n * kPart8 - warp * kStateBlock;
         if (left >= kStateBlock && (this_slot->aligned & kCodes)) {
           Fetched<W, G> one;
           fetch(*this_slot, n, one);
@@ -627,25 +630,25 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     if (tab.count == 0) break;
     tab.chunks = (unsigned)chunks;
     // Behind the norm's launch: while it is still running.
-    const auto start = [&](void (*kernel)(AdamTable<CAP>), unsigned blocks) {
+    const auto start = [&](void (*kernel)(AdamTable<CAP>), unsigned blocks, int threads) {
       if (*early) {
         *early = false;
-        return launch_early(ctx->stream, blocks, kernel, tab);
+        return launch_early(ctx->stream, blocks, threads, kernel, tab);
       }
-      kernel<<<blocks, kOptThreads, 0, ctx->stream>>>(tab);
+      kernel<<<blocks, threads, 0, ctx->stream>>>(tab);
       return cudaSuccess;
     };
     DR_TB(ctx);
     if (BITS == 32) {
       const unsigned blocks = std::min(tab.chunks, (unsigned)ctx->num_sms * 4);
-      DR_CUDA(ctx, start(k_adamw<P, G, MASTER, CAP>, blocks), "adamw");
+      DR_CUDA(ctx, start(k_adamw<P, G, MASTER, CAP>, blocks, kOptThreads), "adamw");
     } else {
       auto* kernel = k_adamw8<P, G, MASTER, CAP>;
       // One wave of blocks that stay.
       int resident = 0;
-      DR_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kOptThreads, 0), "adamw8");
+      DR_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads8, 0), "adamw8");
       const unsigned blocks = std::min(tab.chunks, (unsigned)(ctx->num_sms * std::max(resident, 1)));
-      DR_CUDA(ctx, start(kernel, blocks), "adamw8");
+      DR_CUDA(ctx, start(kernel, blocks, kThreads8), "adamw8");
     }
     DR_LAUNCHED(ctx, BITS == 32 ? "adamw" : "adamw8");
   }

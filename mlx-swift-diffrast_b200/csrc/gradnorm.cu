@@ -255,7 +255,7 @@ dr_status launch_scale(dr_ctx* ctx, const dr_grad_tensor* g, int count, const do
     const unsigned blocks = std::min(tab.chunks, 2 * most_blocks(ctx));
     DR_TB(ctx);
     if (first)
-      DR_CUDA(ctx, launch_early(ctx->stream, blocks, k_clip_scale<CAP>, tab, work, parts, max_norm, norm), "clip_scale");
+      DR_CUDA(ctx, launch_early(ctx->stream, blocks, kOptThreads, k_clip_scale<CAP>, tab, work, parts, max_norm, norm), "clip_scale");
     else
       k_clip_scale<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work, parts, max_norm, norm);
     first = false;
@@ -268,7 +268,7 @@ dr_status launch_scale(dr_ctx* ctx, const dr_grad_tensor* g, int count, const do
 
 dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* norm) {
   DR_TB(ctx);
-  DR_CUDA(ctx, launch_early(ctx->stream, 1, k_grad_norm_finish, work, parts, norm), "grad_norm_finish");
+  DR_CUDA(ctx, launch_early(ctx->stream, 1, kOptThreads, k_grad_norm_finish, work, parts, norm), "grad_norm_finish");
   DR_LAUNCHED(ctx, "grad_norm_finish");
   return DR_OK;
 }

@@ -141,9 +141,10 @@ __device__ __forceinline__ int tensor_of(const unsigned* first, int count, unsig
 constexpr int kOptWarps = kOptThreads / 32;
 constexpr int kRounds = 3;
 
-// Sum over the block in a fixed order; every thread gets it.  kOptThreads threads.
+// Sum over the block in a fixed order; every thread gets it.
+template <int THREADS = kOptThreads>
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double s_warp[kOptThreads / 32];
+  __shared__ double s_warp[THREADS / 32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();  // s_warp may still be read from an earlier call
@@ -151,16 +152,19 @@ __device__ __forceinline__ double block_sum(double v) {
   __syncthreads();
   double s = 0.0;
 #pragma unroll
-  for (int i = 0; i < kOptThreads / 32; ++i) s += s_warp[i];
+  for (int i = 0; i < THREADS / 32; ++i) s += s_warp[i];
   return s;
 }
 
 // The norm that `count` partial sums of squares give: the same value in every
 // block that asks, whatever its place.
+template <int THREADS = kOptThreads>
 __device__ __forceinline__ double norm_of(const double* part, int count) {
+  // Added in the same order whatever the block's size: by the first kOptThreads threads.
   double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += kOptThreads) s += part[i];
-  return sqrt(block_sum(s));
+  if (threadIdx.x < kOptThreads)
+    for (int i = threadIdx.x; i < count; i += kOptThreads) s += part[i];
+  return sqrt(block_sum<THREADS>(s));
 }
 
 // min(1, max_norm / (norm + 1e-6)); a NaN stays one.
@@ -172,13 +176,14 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
 // Launches `kernel`, which calls after_previous(), while the launch before it on
 // the stream is still running.
 template <typename... Params, typename... Args>
-inline cudaError_t launch_early(cudaStream_t stream, unsigned blocks, void (*kernel)(Params...), Args&&... args) {
+inline cudaError_t launch_early(cudaStream_t stream, unsigned blocks, int threads, void (*kernel)(Params...),
+                                Args&&... args) {
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(blocks);
-  config.blockDim = dim3(kOptThreads);
+  config.blockDim = dim3((unsigned)threads);
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;
