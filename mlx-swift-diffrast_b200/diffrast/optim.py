@@ -259,7 +259,7 @@ class AdamW:
         _check_apart(self.params, "AdamW")
         if lr_device is not None and lr_device.device != self.params[0].device:
             raise ValueError("AdamW: a learning_rate tensor must be on the parameters' device")
-        decays = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else list(weight_decay)
+        decays = [float(weight_decay)] * count if np.ndim(weight_decay) == 0 else list(weight_decay)
         ratios = [1.0] * count if lr_ratios is None else list(lr_ratios)
         for name, v in (("weight_decay", decays), ("lr_ratios", ratios)):
             if len(v) != count:
@@ -307,7 +307,7 @@ class AdamW:
         self._tab = tab
         # A step updates the memory that it was given: these keep it alive, and
         # the parameters must still be there.
-        self._held = [p.detach() for p in self.params]
+        self._held = [p.detach() for p in self.params] + list(self.state.values())
         self._addresses = tab["param"][:] = [p.data_ptr() for p in self.params]
         self._index, self._device, self._context = dev.index, dev, _context(dev.index)
         with torch.cuda.device(dev):
@@ -370,8 +370,8 @@ class AdamW:
         """One step from `grads` (one for each parameter, or None to leave it as
         it is; default: the parameters' .grad).  Gradients have their parameter's
         shape and type, or one of the two is float32; they share no memory with
-        other parameters.  Returns the norm of the
-        gradients (a float32 scalar on the device) with max_grad_norm, else None."""
+        other parameters.  Returns the norm of the gradients (a float32 scalar
+        on the device) with max_grad_norm, else None."""
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.step(grads)
