@@ -517,6 +517,12 @@ typedef struct dr_grad_tensor {
  * captured graphs) each need their own. */
 DR_API size_t dr_grad_norm_work_bytes(const dr_ctx* ctx, int count);
 
+/* A list of at most so many tensors, whose sizes, each rounded up to a multiple
+ * of 2048, sum to at most so many elements, needs no `work` in dr_grad_norm
+ * (NULL). */
+#define DR_GRAD_NORM_SMALL_COUNT 64
+#define DR_GRAD_NORM_SMALL_ELEMENTS 16384
+
 /* *norm (device) = the 2-norm over all elements of `count` tensors, of any mix
  * of types.  Squares are formed and summed in 64 bits in a fixed order, so the
  * result neither overflows before the norm itself does nor changes from run to

@@ -27,8 +27,8 @@ struct GradEntry {
 // A launch carries its list as a parameter, which a captured graph keeps: no
 // table in device memory that a replay would have to find unchanged.  The block
 // comes in three sizes: the host copies all of it at each launch, and 28 KB of
-// it cost 2 us where 2 KB cost next to nothing (the norm of two small tensors:
-// 13.5 us with the small block, 15.7 with the large one).
+// it cost 2 us where 2 KB cost next to nothing (the norm of two small tensors,
+// 13.5 us with the small block at the time, took 15.7 with the large one).
 template <int CAP>
 struct GradTable {
   GradEntry t[CAP];
@@ -237,8 +237,9 @@ dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* 
     if (tab.count == 0) break;
     const unsigned blocks = norm ? 1 : std::min(tab.chunks, most_blocks(ctx));
     DR_TB(ctx);
-    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, work + *parts, norm);
+    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, norm ? nullptr : work + *parts, norm);
     DR_LAUNCHED(ctx, "grad_norm_parts");
+    if (norm) return DR_OK;
     *parts += (int)blocks;
   }
   return DR_OK;
@@ -294,15 +295,18 @@ size_t dr_grad_norm_work_bytes(const dr_ctx* ctx, int count) {
 
 dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, float* norm, void* work) {
   DR_ENTER(ctx);
-  DR_REQUIRE(ctx, norm && work && ((uintptr_t)work & 7) == 0, "grad_norm: norm and an 8-byte aligned work are required");
+  DR_REQUIRE(ctx, norm, "grad_norm: norm is required");
   dr_status st = check_list(ctx, grads, count, "grad_norm");
   if (st != DR_OK) return st;
-  // The whole of a list of one block is formed in its one launch.
+  // The norm of a list of one block is formed in its one launch.
   int parts = 0;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) chunks += opt_chunks(grads[i].n);
-  const bool one = chunks > 0 && chunks <= kOptWarps && count <= kSmall;
-  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, one ? norm : nullptr)) != DR_OK || one) return st;
+  static_assert(DR_GRAD_NORM_SMALL_COUNT == kSmall && DR_GRAD_NORM_SMALL_ELEMENTS == kOptWarps * kOptChunk, "as stated");
+  const bool one = chunks <= kOptWarps && count <= kSmall;
+  DR_REQUIRE(ctx, one || (work && ((uintptr_t)work & 7) == 0), "grad_norm: an 8-byte aligned work is required");
+  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, one ? norm : nullptr)) != DR_OK) return st;
+  if (one && chunks > 0) return DR_OK;
   return grad_norm_finish(ctx, (const double*)work, parts, norm);
 }
 

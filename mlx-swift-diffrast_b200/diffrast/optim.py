@@ -158,8 +158,8 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
         ts = [t if t.is_contiguous() else dense(t) for t in _check_list(ts, what)]
         if max_norm > 0.0:
             _check_apart(ts, what)
-        found = ts[0].get_device(), _grad_table(ts).tobytes()
-    index, rows = found
+        found = ts[0].get_device(), _grad_table(ts).tobytes(), True
+    index, rows, large = found
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _norm_call(ts, what, max_norm, dense)
@@ -167,8 +167,8 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
     # From torch's allocator at each call: both belong to the stream (or to the
     # graph being captured) and to no other call.
     norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
-    work = _norm_work(index, len(ts))
-    status = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), work.data_ptr())
+    work = _norm_work(index, len(ts)) if large or max_norm > 0.0 else None
+    status = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), None if work is None else work.data_ptr())
     if status:
         L.check(status, c, what)
     return norm

@@ -93,8 +93,8 @@ PyObject** items(PyObject* o, Py_ssize_t& n) {
   return PySequence_Fast_ITEMS(o);
 }
 
-// grads(tensors, apart) -> (device index, dr_grad_tensor rows as bytes), or
-// None.  apart: also None where two tensors share memory.
+// grads(tensors, apart) -> (device index, dr_grad_tensor rows as bytes, whether
+// the norm needs work), or None.  apart: also None where two tensors share memory.
 PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_ssize_t n = 0;
   PyObject** it = nargs == 2 ? items(args[0], n) : nullptr;
@@ -103,6 +103,7 @@ PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!bytes) return nullptr;
   auto* rows = reinterpret_cast<dr_grad_tensor*>(PyBytes_AS_STRING(bytes));
   int32_t device = -1;
+  int64_t rounded = 0;
   bool fine = true;
   for (Py_ssize_t i = 0; fine && i < n; ++i) {
     Seen s;
@@ -110,6 +111,7 @@ PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!fine) break;
     device = s.t.device.device_id;
     rows[i] = {address(s), s.n, s.type, 0};
+    rounded += (s.n + 2047) / 2048 * 2048;
   }
   if (fine && n > 1 && PyObject_IsTrue(args[1]) == 1) {
     struct Span {
@@ -127,7 +129,8 @@ PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (Py_ssize_t i = 1; i < k; ++i) fine = fine && spans[i - 1].end <= spans[i].begin;
     delete[] spans;
   }
-  PyObject* found = fine ? Py_BuildValue("(iO)", (int)device, bytes) : Py_NewRef(Py_None);
+  const bool small = n <= DR_GRAD_NORM_SMALL_COUNT && rounded <= DR_GRAD_NORM_SMALL_ELEMENTS;
+  PyObject* found = fine ? Py_BuildValue("(iOO)", (int)device, bytes, small ? Py_False : Py_True) : Py_NewRef(Py_None);
   Py_DECREF(bytes);
   return found;
 }
@@ -254,7 +257,7 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyMethodDef methods[] = {
-    {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows) or None"},
+    {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows, needs work) or None"},
     {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
     {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> status"},
     {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads, table, ... -> status or -1"},

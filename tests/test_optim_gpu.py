@@ -700,3 +700,26 @@ def test_c_entries_refuse_bad_rows():
     assert L.dr_grad_norm(c, None, -1, p, work.data_ptr()) == _lib.DR_EINVAL
     torch.cuda.synchronize()
     assert ctypes.sizeof(ctypes.c_void_p) == 8 and bool((x[:256] == 0).all())
+
+
+def test_small_norms_need_no_work_and_large_ones_do():
+    # The bounds that the header names: 64 tensors, 16,384 elements in steps of 2048.
+    from diffrast import _lib
+    L, c = _lib.lib(), _lib.ctx_for(0)
+    x = torch.randn(40_000, device="cuda")
+    norm = torch.zeros((), device="cuda")
+
+    def call(sizes):
+        rows = np.zeros(len(sizes), optim._GRAD_ROW)
+        rows["data"], rows["n"] = x.data_ptr(), sizes
+        return L.dr_grad_norm(c, rows.ctypes.data, len(sizes), norm.data_ptr(), None)
+
+    for sizes in ([16384], [2048] * 8, [1] * 8, [0] * 64 + [], [5] * 7 + [0] * 50, [14336, 1]):
+        assert call(sizes) == _lib.DR_OK
+        ref = math.sqrt(sum(float((f64(x[:n]) ** 2).sum()) for n in sizes))
+        assert abs(float(norm) - ref) <= 1.01 * AO.U * ref, sizes
+    for sizes in ([16385], [2048] * 8 + [1], [1] * 9, [0] * 65, [14337, 1, 1]):
+        assert call(sizes) == _lib.DR_EINVAL
+    for n in (16384, 16385):
+        ref = math.sqrt(float((f64(x[:n]) ** 2).sum()))
+        assert abs(float(optim.grad_norm([x[:n]])) - ref) <= 1.01 * AO.U * ref
