@@ -518,8 +518,8 @@ typedef struct dr_grad_tensor {
 DR_API size_t dr_grad_norm_work_bytes(const dr_ctx* ctx, int count);
 
 /* A list of at most so many tensors, whose sizes, each rounded up to a multiple
- * of 2048, sum to at most so many elements, needs no `work` in dr_grad_norm
- * (NULL). */
+ * of 2048, sum to at most so many elements, needs no `work` (NULL) in
+ * dr_grad_norm and dr_clip_grad_norm, and takes one launch. */
 #define DR_GRAD_NORM_SMALL_COUNT 64
 #define DR_GRAD_NORM_SMALL_ELEMENTS 16384
 

@@ -715,7 +715,7 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
     dr_grad_tensor* g = new (std::nothrow) dr_grad_tensor[(size_t)count + 1];
     if (!g) return fail(ctx, DR_ENOMEM, "adamw: no host memory for %d tensors", count);
     for (int i = 0; i < count; ++i) g[i] = {const_cast<void*>(t[i].grad), t[i].n, t[i].grad_type, 0};
-    const dr_status st = grad_norm_parts(ctx, g, count, (double*)work, &h.parts, nullptr);
+    const dr_status st = grad_norm_parts(ctx, g, count, (double*)work, &h.parts, nullptr, 0.0);
     delete[] g;
     if (st != DR_OK) return st;
     h.part = (const double*)work;

@@ -106,6 +106,27 @@ __device__ __forceinline__ double squares_of(const Fetched& x) {
   return squares<T>(f);
 }
 
+template <typename T>
+__device__ __forceinline__ void scale_vec(const GradSlot& e, float f) {
+  const int valid = min(kOptVec, e.valid - (int)threadIdx.x * kOptVec);
+  if (valid <= 0) return;
+  float x[kOptVec];
+  T* p = (T*)e.data + threadIdx.x * kOptVec;
+  const bool whole = valid == kOptVec && vector_aligned(p);
+  if (whole) load_vec(p, x);
+  else load_some(p, valid, x);
+#pragma unroll
+  for (int i = 0; i < kOptVec; ++i) x[i] = __fmul_rn(x[i], f);
+  if (whole) store_vec(p, x);
+  else store_some(p, valid, x);
+}
+
+__device__ __forceinline__ void scale_chunk(const GradSlot& e, float f) {
+  if (e.type == DR_F32) scale_vec<float>(e, f);
+  else if (e.type == DR_BF16) scale_vec<__nv_bfloat16>(e, f);
+  else scale_vec<__half>(e, f);
+}
+
 // A thread's loads of kAhead chunks are under way together: 22.4 us for the soup
 // with four; 25 with two (and twice the blocks), 31 with eight.
 constexpr int kAhead = 4;
@@ -114,7 +135,7 @@ static_assert(kOptWarps % kAhead == 0, "rounds of whole batches");
 template <int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_constant__ GradTable<CAP> tab,
                                                                  double* __restrict__ part,
-                                                                 float* __restrict__ norm) {
+                                                                 float* __restrict__ norm, double max_norm) {
   __shared__ GradSlot s_slots[kRounds][kOptWarps];
   const unsigned warp = threadIdx.x / 32;
   double s = 0.0;
@@ -144,9 +165,16 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_co
   }
   let_next_start();
   s = block_sum(s);
-  if (threadIdx.x != 0) return;
-  if (norm) *norm = (float)sqrt(s);  // the only block of the only launch
-  else part[blockIdx.x] = s;
+  if (!norm) {
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    return;
+  }
+  // The only block of the only launch: the list is one round, whose slots are still there.
+  s = sqrt(s);
+  if (threadIdx.x == 0) *norm = (float)s;
+  const float f = max_norm > 0.0 ? clip_factor(s, max_norm) : 1.0f;
+  if (f == 1.0f) return;
+  for (unsigned b = 0; b < tab.chunks; ++b) scale_chunk(s_slots[0][b], f);
 }
 
 __global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* __restrict__ part, int count,
@@ -154,21 +182,6 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* 
   after_previous();
   const double s = norm_of(part, count);
   if (threadIdx.x == 0) *norm = (float)s;
-}
-
-template <typename T>
-__device__ __forceinline__ void scale_vec(const GradSlot& e, float f) {
-  const int valid = min(kOptVec, e.valid - (int)threadIdx.x * kOptVec);
-  if (valid <= 0) return;
-  float x[kOptVec];
-  T* p = (T*)e.data + threadIdx.x * kOptVec;
-  const bool whole = valid == kOptVec && vector_aligned(p);
-  if (whole) load_vec(p, x);
-  else load_some(p, valid, x);
-#pragma unroll
-  for (int i = 0; i < kOptVec; ++i) x[i] = __fmul_rn(x[i], f);
-  if (whole) store_vec(p, x);
-  else store_some(p, valid, x);
 }
 
 template <int CAP>
@@ -188,12 +201,7 @@ __global__ void __launch_bounds__(kOptThreads) k_clip_scale(const __grid_constan
   for (int round = 0; c < tab.chunks; round = round + 1 == kRounds ? 0 : round + 1) {
     look_up(tab, c + (kOptWarps + warp) * gridDim.x, s_slots[round + 1 == kRounds ? 0 : round + 1][warp]);
 #pragma unroll 1
-    for (int b = 0; b < kOptWarps && c < tab.chunks; ++b, c += gridDim.x) {
-      const GradSlot& e = s_slots[round][b];
-      if (e.type == DR_F32) scale_vec<float>(e, f);
-      else if (e.type == DR_BF16) scale_vec<__nv_bfloat16>(e, f);
-      else scale_vec<__half>(e, f);
-    }
+    for (int b = 0; b < kOptWarps && c < tab.chunks; ++b, c += gridDim.x) scale_chunk(s_slots[round][b], f);
     __syncthreads();
   }
 }
@@ -214,6 +222,14 @@ dr_status check_list(dr_ctx* ctx, const dr_grad_tensor* g, int count, const char
   return DR_OK;
 }
 
+// A list whose norm one block forms, and by which it scales it, in one launch.
+bool is_small(const dr_grad_tensor* g, int count) {
+  static_assert(DR_GRAD_NORM_SMALL_COUNT == kSmall && DR_GRAD_NORM_SMALL_ELEMENTS == kOptWarps * kOptChunk, "as stated");
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) chunks += opt_chunks(g[i].n);
+  return chunks <= kOptWarps && count <= kSmall;
+}
+
 // The next launch's part of a list, from *i on: at most CAP tensors with elements.
 template <int CAP>
 void fill(const dr_grad_tensor* g, int count, int* i, GradTable<CAP>* tab) {
@@ -230,16 +246,17 @@ void fill(const dr_grad_tensor* g, int count, int* i, GradTable<CAP>* tab) {
 }
 
 template <int CAP>
-dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* work, int* parts, float* norm) {
+dr_status launch_parts(dr_ctx* ctx, const dr_grad_tensor* g, int count, double* work, int* parts, float* norm,
+                       double max_norm) {
   for (int i = 0; i < count;) {
     GradTable<CAP> tab;
     fill(g, count, &i, &tab);
     if (tab.count == 0) break;
     const unsigned blocks = norm ? 1 : std::min(tab.chunks, most_blocks(ctx));
     DR_TB(ctx);
-    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, norm ? nullptr : work + *parts, norm);
+    k_grad_norm_parts<CAP><<<blocks, kOptThreads, 0, ctx->stream>>>(tab, norm ? nullptr : work + *parts, norm,
+                                                                       max_norm);
     DR_LAUNCHED(ctx, "grad_norm_parts");
-    if (norm) return DR_OK;
     *parts += (int)blocks;
   }
   return DR_OK;
@@ -275,11 +292,11 @@ dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* no
 }
 
 dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts,
-                          float* norm) {
+                          float* norm, double max_norm) {
   *parts = 0;
-  return count <= kSmall    ? launch_parts<kSmall>(ctx, grads, count, work, parts, norm)
-         : count <= kMedium ? launch_parts<kMedium>(ctx, grads, count, work, parts, norm)
-                            : launch_parts<kLarge>(ctx, grads, count, work, parts, norm);
+  return count <= kSmall    ? launch_parts<kSmall>(ctx, grads, count, work, parts, norm, max_norm)
+         : count <= kMedium ? launch_parts<kMedium>(ctx, grads, count, work, parts, norm, max_norm)
+                            : launch_parts<kLarge>(ctx, grads, count, work, parts, norm, max_norm);
 }
 
 }  // namespace dr
@@ -298,28 +315,26 @@ dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, floa
   DR_REQUIRE(ctx, norm, "grad_norm: norm is required");
   dr_status st = check_list(ctx, grads, count, "grad_norm");
   if (st != DR_OK) return st;
-  // The norm of a list of one block is formed in its one launch.
+  const bool small = is_small(grads, count);
+  DR_REQUIRE(ctx, small || (work && ((uintptr_t)work & 7) == 0), "grad_norm: an 8-byte aligned work is required");
   int parts = 0;
-  int64_t chunks = 0;
-  for (int i = 0; i < count; ++i) chunks += opt_chunks(grads[i].n);
-  static_assert(DR_GRAD_NORM_SMALL_COUNT == kSmall && DR_GRAD_NORM_SMALL_ELEMENTS == kOptWarps * kOptChunk, "as stated");
-  const bool one = chunks <= kOptWarps && count <= kSmall;
-  DR_REQUIRE(ctx, one || (work && ((uintptr_t)work & 7) == 0), "grad_norm: an 8-byte aligned work is required");
-  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, one ? norm : nullptr)) != DR_OK) return st;
-  if (one && chunks > 0) return DR_OK;
-  return grad_norm_finish(ctx, (const double*)work, parts, norm);
+  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, small ? norm : nullptr, 0.0)) != DR_OK) return st;
+  return small && parts ? DR_OK : grad_norm_finish(ctx, (const double*)work, parts, norm);
 }
 
 dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double max_norm, float* norm,
                             void* work) {
   DR_ENTER(ctx);
-  DR_REQUIRE(ctx, norm && work && ((uintptr_t)work & 7) == 0,
-             "clip_grad_norm: norm and an 8-byte aligned work are required");
+  DR_REQUIRE(ctx, norm, "clip_grad_norm: norm is required");
   DR_REQUIRE(ctx, max_norm > 0.0 && max_norm < 1e300, "clip_grad_norm: max_norm must be positive and finite");
   dr_status st = check_list(ctx, grads, count, "clip_grad_norm");
   if (st != DR_OK) return st;
+  const bool small = is_small(grads, count);
+  DR_REQUIRE(ctx, small || (work && ((uintptr_t)work & 7) == 0), "clip_grad_norm: an 8-byte aligned work is required");
   int parts = 0;
-  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, nullptr)) != DR_OK) return st;
+  if ((st = grad_norm_parts(ctx, grads, count, (double*)work, &parts, small ? norm : nullptr, max_norm)) != DR_OK)
+    return st;
+  if (small && parts) return DR_OK;
   if (parts == 0) return grad_norm_finish(ctx, (const double*)work, 0, norm);  // nothing to scale
   const double* part = (const double*)work;
   return count <= kSmall    ? launch_scale<kSmall>(ctx, grads, count, part, parts, max_norm, norm)

@@ -196,8 +196,10 @@ __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.
 
 bool valid_type(int type);
 // Launches the partial sums of squares of a list; *parts of them lie in `work`.
-// With `norm`, for a list of one launch: one block forms the norm itself.
-dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts, float* norm);
+// With `norm`, for a list of one round of one block: it forms the norm itself,
+// and with max_norm > 0 clips the gradients by it.
+dr_status grad_norm_parts(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double* work, int* parts, float* norm,
+                          double max_norm);
 // *norm = the norm that the partial sums give.
 dr_status grad_norm_finish(dr_ctx* ctx, const double* work, int parts, float* norm);
 

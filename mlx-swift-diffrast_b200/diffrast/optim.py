@@ -167,7 +167,7 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
     # From torch's allocator at each call: both belong to the stream (or to the
     # graph being captured) and to no other call.
     norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
-    work = _norm_work(index, len(ts)) if large or max_norm > 0.0 else None
+    work = _norm_work(index, len(ts)) if large else None
     status = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), None if work is None else work.data_ptr())
     if status:
         L.check(status, c, what)

@@ -723,3 +723,19 @@ def test_small_norms_need_no_work_and_large_ones_do():
     for n in (16384, 16385):
         ref = math.sqrt(float((f64(x[:n]) ** 2).sum()))
         assert abs(float(optim.grad_norm([x[:n]])) - ref) <= 1.01 * AO.U * ref
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sizes", [[5], [2048] * 8, [16384], [1, 0, 300, 7] * 2, [16385], [2048] * 8 + [1]])
+def test_clip_in_one_block_and_in_more(dtype, sizes):
+    rng = np.random.default_rng(sum(sizes))
+    gs = [(grads_like(rng, n + 1, dtype) + 0)[i % 2:][:n] for i, n in enumerate(sizes)]
+    old = [f64(g) for g in gs]
+    ref = math.sqrt(sum(float((x ** 2).sum()) for x in old))
+    for top in (2 * ref + 1, 0.3 * ref + 1e-4):
+        got = optim.clip_grad_norm_(gs, top)
+        assert abs(float(got) - ref) <= 1.01 * AO.U * ref
+    c = AO.clip_factor(ref, top)
+    for g, x in zip(gs, old):
+        y = x * c
+        assert np.all(np.abs(f64(g) - y) <= (2 * AO.U + HALF[dtype]) * np.abs(y) * (1 + 4 * AO.U) + 2.0 ** -25)
