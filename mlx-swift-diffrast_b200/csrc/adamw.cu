@@ -617,15 +617,15 @@ dr_status launch(dr_ctx* ctx, const dr_adamw_tensor* t, int count, const AdamHyp
     for (; i < count && tab.count < CAP; ++i) {
       const dr_adamw_tensor& x = t[i];
       if (x.n == 0 || x.param_type != pt || x.grad_type != gt || (x.master != nullptr) != MASTER) continue;
-      const bool states = BITS == 8 || (vector_aligned((const float*)x.m) && vector_aligned((const float*)x.v));
-      const bool vectors = vector_aligned((const P*)x.param) && vector_aligned((const G*)x.grad) &&
-                           (!MASTER || vector_aligned(x.master)) && states;
-      const bool codes = BITS == 8 && (((uintptr_t)x.m | (uintptr_t)x.v) & 7) == 0;
-      const int aligned = (vectors ? kVectors : 0) | (codes ? kCodes : 0);
-      tab.first[tab.count] = (unsigned)chunks;
+      AdamEntry& e = tab.t[tab.count];
+      e = {x.param, x.grad, x.master, x.m, x.v, x.m_scale, x.v_scale, x.n, x.lr_ratio, x.weight_decay, x.seed, 0};
+      if (vector_aligned((const P*)x.param) && vector_aligned((const G*)x.grad) &&
+          (!MASTER || vector_aligned(x.master)) &&
+          (BITS == 8 || (vector_aligned((const float*)x.m) && vector_aligned((const float*)x.v))))
+        e.aligned |= kVectors;
+      if (BITS == 8 && (((uintptr_t)x.m | (uintptr_t)x.v) & 7) == 0) e.aligned |= kCodes;
       tab.clock[tab.count] = x.clock;
-      tab.t[tab.count++] = {x.param,   x.grad, x.master,   x.m,            x.v,    x.m_scale,
-                            x.v_scale, x.n,    x.lr_ratio, x.weight_decay, x.seed, aligned};
+      tab.first[tab.count++] = (unsigned)chunks;
       chunks += BITS == 32 ? opt_chunks(x.n) : (x.n + kChunk8 - 1) / kChunk8;
     }
     if (tab.count == 0) break;
