@@ -177,8 +177,10 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_parts(const __grid_co
   for (unsigned b = 0; b < tab.chunks; ++b) scale_chunk(s_slots[0][b], f);
 }
 
-__global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* __restrict__ part, int count,
-                                                                  float* __restrict__ norm) {
+// `part` of the two kernels below is written by the launch before them while
+// they are resident already: a plain pointer, so that its loads are ordinary
+// (coherent) ones, which the wait's memory clobber holds behind it.
+__global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* part, int count, float* norm) {
   after_previous();
   const double s = norm_of(part, count);
   if (threadIdx.x == 0) *norm = (float)s;
@@ -186,8 +188,8 @@ __global__ void __launch_bounds__(kOptThreads) k_grad_norm_finish(const double* 
 
 template <int CAP>
 __global__ void __launch_bounds__(kOptThreads) k_clip_scale(const __grid_constant__ GradTable<CAP> tab,
-                                                            const double* __restrict__ part, int parts,
-                                                            double max_norm, float* __restrict__ norm) {
+                                                            const double* part, int parts, double max_norm,
+                                                            float* norm) {
   __shared__ GradSlot s_slots[kRounds][kOptWarps];
   const unsigned warp = threadIdx.x / 32;
   unsigned c = blockIdx.x;
