@@ -490,15 +490,22 @@ __device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
   return isfinite(norm);  // the same in every block
 }
 
+// One more to *count, and what it was.  Released and acquired: the reads that a
+// block did before its barrier are behind it for whoever draws a later number.
+__device__ __forceinline__ uint32_t draw(uint32_t* count) {
+  uint32_t was;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(was) : "l"(count) : "memory");
+  return was;
+}
+
 // The last block to come here has every other block's reads of the clocks
-// behind it (their values were used before its ticket was drawn, so no fence is
-// needed): it advances them, and leaves the ticket as it found it.
+// behind it: it advances them, and leaves the ticket as it found it.
 template <int CAP>
 __device__ __forceinline__ void end_step(const AdamTable<CAP>& tab) {
   const AdamHyper& h = tab.h;
   __shared__ bool s_last;
   __syncthreads();
-  if (threadIdx.x == 0) s_last = gridDim.x == 1 || atomicAdd(h.ticket, 1u) == gridDim.x - 1;
+  if (threadIdx.x == 0) s_last = gridDim.x == 1 || draw(h.ticket) == gridDim.x - 1;
   __syncthreads();
   if (!s_last) return;
   for (int i = threadIdx.x; i < tab.count; i += blockDim.x) {

@@ -33,3 +33,10 @@ def test_no_other_file_launches_early():
     for path in glob.glob(os.path.join(CSRC, "*")):
         if os.path.basename(path) not in ("gradnorm.cu", "adamw.cu", "optim_common.cuh"):
             assert "griddepcontrol" not in open(path).read() and "launch_early" not in open(path).read(), path
+
+
+def test_the_clocks_last_block_is_ordered_behind_the_others_reads():
+    # Other blocks' plain reads of the clocks and the last block's writes need an order of the memory model's.
+    body = {re.sub(r"\(.*", "", s, flags=re.S).split()[-1]: b for s, b in functions("adamw.cu")}
+    assert "draw(h.ticket)" in body["end_step"] and "atomicAdd" not in body["end_step"]
+    assert "atom.acq_rel.gpu" in body["draw"] and '"memory"' in body["draw"]
