@@ -81,7 +81,8 @@ SIGNATURES = {
 
 _lib = None
 _lock = threading.RLock()
-_ctx = {}
+_ctx = {}  # device index -> the context of the render operators and Adam
+_lists = {}  # device index -> the context of the optimizer's lists, whose calls take turns in diffrast._rows
 
 
 class DiffRastError(RuntimeError):
@@ -106,6 +107,14 @@ def lib():
     return _lib
 
 
+def _create(device_index: int):
+    h = P()
+    st = lib().dr_ctx_create(device_index, ctypes.byref(h))
+    if st != DR_OK:
+        raise DiffRastError(f"dr_ctx_create({device_index}) -> {_STATUS.get(st, st)}")
+    return h
+
+
 def ctx_for(device_index: int):
     """Per-device context (created on first use, kept for the process)."""
     c = _ctx.get(device_index)
@@ -114,52 +123,64 @@ def ctx_for(device_index: int):
         with _lock:
             c = _ctx.get(device_index)
             if c is None:
-                h = P()
-                st = lib().dr_ctx_create(device_index, ctypes.byref(h))
-                if st != DR_OK:
-                    raise DiffRastError(f"dr_ctx_create({device_index}) -> {_STATUS.get(st, st)}")
-                c = h
+                c = _create(device_index)
+                # With it, since a stream capture that calls the optimizer first must create nothing.
+                _lists[device_index] = _create(device_index)
                 _ctx[device_index] = c
     return c
+
+
+def lists_ctx_for(device_index: int):
+    """The device's context of grad_norm, clip_grad_norm_ and AdamW: their own, so that no operator of another thread
+    moves it to another stream between a call's launches."""
+    ctx_for(device_index)
+    return _lists[device_index]
+
+
+def _contexts(device_index: int):
+    return ctx_for(device_index), _lists[device_index]
+
+
+def failed(st: int, msg: str, what: str):
+    err = DiffRastError(f"{what}: {_STATUS.get(st, st)}: {msg}")
+    err.status = st
+    raise err
 
 
 def check(st: int, ctx, what: str):
     if st != DR_OK:
         msg = lib().dr_last_error(ctx)
-        msg = msg.decode() if msg else ""
-        err = DiffRastError(f"{what}: {_STATUS.get(st, st)}: {msg}")
-        err.status = st
-        raise err
+        failed(st, msg.decode() if msg else "", what)
 
 
 def launch_count(device_index: int = 0) -> int:
-    return int(lib().dr_ctx_launch_count(ctx_for(device_index)))
+    return sum(int(lib().dr_ctx_launch_count(c)) for c in _contexts(device_index))
 
 
 def workspace_bytes(device_index: int = 0) -> int:
-    return int(lib().dr_ctx_workspace_bytes(ctx_for(device_index)))
+    return sum(int(lib().dr_ctx_workspace_bytes(c)) for c in _contexts(device_index))
 
 
 def set_timing(enable: bool, device_index: int = 0):
-    c = ctx_for(device_index)
-    check(lib().dr_ctx_set_timing(c, 1 if enable else 0), c, "dr_ctx_set_timing")
+    for c in _contexts(device_index):
+        check(lib().dr_ctx_set_timing(c, 1 if enable else 0), c, "dr_ctx_set_timing")
 
 
 def timing_report(device_index: int = 0) -> dict:
     """{kernel name: (launches, total ms)} since timing was enabled."""
-    c = ctx_for(device_index)
-    buf = ctypes.create_string_buffer(1 << 16)
-    check(lib().dr_ctx_timing_report(c, buf, len(buf)), c, "dr_ctx_timing_report")
     out = {}
-    for line in buf.value.decode().splitlines():
-        name, cnt, ms = line.split()
-        out[name] = (int(cnt), float(ms))
+    for c in _contexts(device_index):
+        buf = ctypes.create_string_buffer(1 << 16)
+        check(lib().dr_ctx_timing_report(c, buf, len(buf)), c, "dr_ctx_timing_report")
+        for line in buf.value.decode().splitlines():
+            name, cnt, ms = line.split()
+            out[name] = (int(cnt), float(ms))
     return out
 
 
 def sync(device_index: int = 0):
-    c = ctx_for(device_index)
-    check(lib().dr_ctx_sync(c), c, "dr_ctx_sync")
+    for c in _contexts(device_index):
+        check(lib().dr_ctx_sync(c), c, "dr_ctx_sync")
 
 
 def set_raster_list_capacity(pairs: int, device_index: int = 0):

@@ -133,11 +133,12 @@ def _written(ts) -> None:
 
 @functools.lru_cache(maxsize=None)
 def _context(index: int) -> int:
-    """The address of a device's context; binds the library's functions at the first call."""
-    c = L.ctx_for(index)
+    """The address of the device's context of this module's lists; binds the library's functions at the first call."""
+    c = L.lists_ctx_for(index)
     lib = L.lib()
     _rows.bind(*(ctypes.cast(f, ctypes.c_void_p).value
-                 for f in (lib.dr_ctx_set_stream, lib.dr_grad_norm, lib.dr_clip_grad_norm, lib.dr_adamw_step)))
+                 for f in (lib.dr_ctx_set_stream, lib.dr_last_error, lib.dr_grad_norm, lib.dr_clip_grad_norm,
+                           lib.dr_adamw_step)))
     return c.value
 
 
@@ -168,9 +169,9 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
     # graph being captured) and to no other call.
     norm = torch.empty((), dtype=torch.float32, device=_CUDA[index])
     work = _norm_work(index, len(ts)) if large else None
-    status = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), None if work is None else work.data_ptr())
-    if status:
-        L.check(status, c, what)
+    error = _rows.norm(c, index, rows, max_norm, norm.data_ptr(), None if work is None else work.data_ptr())
+    if error:
+        L.failed(*error, what)
     return norm
 
 
@@ -232,7 +233,8 @@ class AdamW:
 
     t is counted for each parameter on the device, so a captured step (CUDA
     graph) replays as the next one.  Parameters whose gradient is None are left
-    as they are.  Steps of one optimizer must not run at the same time.
+    as they are.  Steps of one optimizer must not run at the same time; those
+    of different ones may, from any threads and on any streams.
     """
 
     def __init__(self, params, learning_rate: Union[float, torch.Tensor] = 1e-3, beta1: float = 0.9,
@@ -384,8 +386,8 @@ class AdamW:
                 self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(), self._work_at,
                 self._ticket_at)
         at = ps
-        status = _rows.step(ps, grads, self._tab, *args)
-        if status < 0:
+        error = _rows.step(ps, grads, self._tab, *args)
+        if error is False:
             gs = [p.grad for p in ps] if grads is None else list(grads)
             if len(gs) != len(ps):
                 raise ValueError(f"AdamW: {len(ps)} gradients expected (got {len(gs)})")
@@ -396,9 +398,9 @@ class AdamW:
             at, gs, table = [ps[i] for i in keep], [gs[i] for i in keep], self._tab[keep]
             table["grad"] = [g.data_ptr() for g in gs]
             table["grad_type"] = [_TYPES[g.dtype] for g in gs]
-            status = _rows.step(None, None, table.tobytes(), *args)
-        if status:
-            L.check(status, self._context, "AdamW")
+            error = _rows.step(None, None, table.tobytes(), *args)
+        if error:
+            L.failed(*error, "AdamW")
         _written(at)
         return norm
 

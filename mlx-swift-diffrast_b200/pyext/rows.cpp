@@ -6,13 +6,15 @@
 // small ones; here it is 0.1 us.  Tensors are read through the DLPack exchange
 // functions that torch.Tensor publishes, so nothing of torch is linked.  The look
 // at the lists answers only for lists that are simple (dense, contiguous, of known
-// types, on one CUDA device) and otherwise returns None or -1, upon which the
+// types, on one CUDA device) and otherwise returns None or False, upon which the
 // Python side looks at the tensors one by one and raises or copies.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdio>
+#include <mutex>
 #include <new>
 
 #include "diffrast.h"
@@ -138,18 +140,20 @@ PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // The C ABI's functions, from the binding that has loaded the library: called
 // from here they cost 2 us less than through ctypes.
 decltype(&dr_ctx_set_stream) set_stream = nullptr;
+decltype(&dr_last_error) last_error = nullptr;
 decltype(&dr_grad_norm) grad_norm = nullptr;
 decltype(&dr_clip_grad_norm) clip_grad_norm = nullptr;
 decltype(&dr_adamw_step) adamw_step = nullptr;
 
-// bind(dr_ctx_set_stream, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step): their addresses.
+// bind(dr_ctx_set_stream, dr_last_error, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step): their addresses.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a, b, c, d;
-  if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return nullptr;
+  unsigned long long a, b, c, d, e;
+  if (!PyArg_ParseTuple(args, "KKKKK", &a, &b, &c, &d, &e)) return nullptr;
   set_stream = reinterpret_cast<decltype(set_stream)>(a);
-  grad_norm = reinterpret_cast<decltype(grad_norm)>(b);
-  clip_grad_norm = reinterpret_cast<decltype(clip_grad_norm)>(c);
-  adamw_step = reinterpret_cast<decltype(adamw_step)>(d);
+  last_error = reinterpret_cast<decltype(last_error)>(b);
+  grad_norm = reinterpret_cast<decltype(grad_norm)>(c);
+  clip_grad_norm = reinterpret_cast<decltype(clip_grad_norm)>(d);
+  adamw_step = reinterpret_cast<decltype(adamw_step)>(e);
   Py_RETURN_NONE;
 }
 
@@ -158,19 +162,38 @@ T* pointer(PyObject* o) {
   return o == Py_None ? nullptr : static_cast<T*>(PyLong_AsVoidPtr(o));
 }
 
-// Puts the context on torch's current stream of the device; false with an exception set.
-bool on_current_stream(dr_ctx* ctx, long device) {
-  void* stream = nullptr;
-  if (api->current_work_stream(kCuda, (int32_t)device, &stream) != 0) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "no current stream");
-    return false;
-  }
-  set_stream(ctx, stream);
-  return true;
+// Torch's current stream of the device; false with an exception set.
+bool current_stream(long device, void** stream) {
+  if (api->current_work_stream(kCuda, (int32_t)device, stream) == 0) return true;
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "no current stream");
+  return false;
 }
 
-// norm(ctx, device, rows, max_norm, norm, work) -> status: dr_grad_norm, or with max_norm > 0 dr_clip_grad_norm,
-// of the rows (bytes) that grads() or the Python side made.
+// A context serves one call at a time, and keeps the stream and the last error
+// of it.  These contexts are used from here alone, and a call of any thread has
+// its turn from setting the stream to copying the error; it waits for it and
+// launches without the GIL.
+std::mutex turn;
+
+// None, or (status, message).
+template <typename Call>
+PyObject* launch(dr_ctx* ctx, void* stream, Call call) {
+  dr_status st;
+  char text[512] = "";
+  Py_BEGIN_ALLOW_THREADS
+  {
+    std::lock_guard<std::mutex> mine(turn);
+    set_stream(ctx, stream);
+    st = call();
+    if (st != DR_OK) snprintf(text, sizeof text, "%s", last_error(ctx));
+  }
+  Py_END_ALLOW_THREADS
+  if (st == DR_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(is)", (int)st, text);
+}
+
+// norm(ctx, device, rows, max_norm, norm, work) -> None or (status, message): dr_grad_norm, or with max_norm > 0
+// dr_clip_grad_norm, of the rows (bytes) that grads() or the Python side made.
 PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 6 || !PyBytes_Check(args[2]) || !set_stream) {
     PyErr_SetString(PyExc_TypeError, "norm(ctx, device, rows, max_norm, norm, work)");
@@ -183,18 +206,18 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const double max_norm = PyFloat_AsDouble(args[3]);
   auto* out = pointer<float>(args[4]);
   auto* work = pointer<void>(args[5]);
-  if (PyErr_Occurred() || !on_current_stream(ctx, device)) return nullptr;
-  dr_status st;
-  Py_BEGIN_ALLOW_THREADS
-  st = max_norm > 0.0 ? clip_grad_norm(ctx, rows, count, max_norm, out, work) : grad_norm(ctx, rows, count, out, work);
-  Py_END_ALLOW_THREADS
-  return PyLong_FromLong(st);
+  void* stream = nullptr;
+  if (PyErr_Occurred() || !current_stream(device, &stream)) return nullptr;
+  return launch(ctx, stream, [&] {
+    return max_norm > 0.0 ? clip_grad_norm(ctx, rows, count, max_norm, out, work)
+                          : grad_norm(ctx, rows, count, out, work);
+  });
 }
 
 // step(params, grads, table, device, ctx, lr, lr_device, beta1, beta2, eps, bits, max_norm, norm, work, ticket)
-// -> status, or -1.  Looks each parameter (its address is its row's, see below) and gradient over, fills the rows'
-// grad and grad_type and calls dr_adamw_step.  grads None: the parameters' .grad.  params None: the rows (bytes)
-// are filled, and -1 does not come back.
+// -> None or (status, message), or False.  Looks each parameter (its address is its row's, see below) and gradient
+// over, fills the rows' grad and grad_type and calls dr_adamw_step.  grads None: the parameters' .grad.  params None:
+// the rows (bytes) are filled, and False does not come back.
 PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 15 || !set_stream) {
     PyErr_SetString(PyExc_TypeError, "step: 15 arguments");
@@ -215,7 +238,7 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool ready = args[0] == Py_None;
   PyObject** ps = ready ? nullptr : items(args[0], n);
   PyObject** gs = args[1] != Py_None ? items(args[1], ng) : nullptr;
-  if (!ready && (!ps || (args[1] != Py_None && (!gs || ng != n)))) return PyLong_FromLong(-1);
+  if (!ready && (!ps || (args[1] != Py_None && (!gs || ng != n)))) Py_RETURN_FALSE;
   if (PyObject_GetBuffer(args[2], &table, ready ? PyBUF_SIMPLE : PyBUF_WRITABLE) != 0) return nullptr;
   if (ready) n = table.len / (Py_ssize_t)sizeof(dr_adamw_tensor);
   bool fine = table.len >= n * (Py_ssize_t)sizeof(dr_adamw_tensor);
@@ -242,25 +265,23 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (!gs) Py_DECREF(grad);  // the parameter holds it
   }
-  long st = -1;
-  bool error = false;
-  if (fine) {
-    error = !on_current_stream(ctx, device);
-    if (!error) {
-      Py_BEGIN_ALLOW_THREADS
-      st = adamw_step(ctx, rows, (int)n, lr, lr_device, beta1, beta2, eps, bits, max_norm, out, work, ticket);
-      Py_END_ALLOW_THREADS
-    }
-  }
+  PyObject* result = nullptr;
+  void* stream = nullptr;
+  if (!fine)
+    result = Py_NewRef(Py_False);
+  else if (current_stream(device, &stream))
+    result = launch(ctx, stream, [&] {
+      return adamw_step(ctx, rows, (int)n, lr, lr_device, beta1, beta2, eps, bits, max_norm, out, work, ticket);
+    });
   PyBuffer_Release(&table);
-  return error ? nullptr : PyLong_FromLong(st);
+  return result;
 }
 
 PyMethodDef methods[] = {
     {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows, needs work) or None"},
-    {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
-    {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> status"},
-    {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads, table, ... -> status or -1"},
+    {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_last_error, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
+    {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> None or (status, message)"},
+    {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads, table, ... -> None, (status, message) or False"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", "Tensors to the C ABI's rows.", -1, methods,

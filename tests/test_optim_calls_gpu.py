@@ -1,0 +1,143 @@
+"""Calls of grad_norm, clip_grad_norm_ and AdamW that their documentation allows and that are easy to get wrong:
+threads, streams, lazily negated tensors, norms beyond float32, lists with gaps, betas and eps of every kind."""
+import math
+import os
+import subprocess
+import sys
+import textwrap
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import adamw_oracle as AO
+from conftest import ROOT
+from diffrast import optim
+
+pytestmark = pytest.mark.gpu
+
+
+def fresh_python(code):
+    """Runs `code` in a process of its own."""
+    paths = os.pathsep.join([ROOT, os.path.join(ROOT, "mlx-swift-diffrast_b200"), os.path.join(ROOT, "tests")])
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": paths})
+    assert r.returncode == 0, r.stdout + r.stderr
+    return r.stdout
+
+
+# ----------------------------------------------------------------- threads
+
+def test_a_calls_launches_see_its_own_stream_whatever_other_threads_call():
+    # The library's entries replaced by ones that look at the stream, wait and look again, and launch nothing: another
+    # thread's call on another stream, of the same functions or of a render operator, must not come in between.
+    out = fresh_python("""
+        import ctypes, threading, time
+        import torch
+        from diffrast import _lib, ops, optim
+        torch.zeros(1, device="cuda")
+        real, here, at, torn, calls = _lib.lib(), threading.local(), {}, [], []
+
+        def set_stream(ctx, stream):
+            at[ctx] = stream
+            return 0
+
+        def norm(ctx, rows, count, out, work):
+            a = at[ctx]
+            time.sleep(0.002)
+            calls.append(1)
+            if a != here.stream or at[ctx] != here.stream:
+                torn.append((a, at[ctx], here.stream))
+            return 0
+
+        class Library:
+            dr_ctx_set_stream = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)(set_stream)
+            dr_grad_norm = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                            ctypes.c_void_p, ctypes.c_void_p)(norm)
+            def __getattr__(self, name):
+                return getattr(real, name)
+
+        _lib._lib = Library()
+        x = torch.ones(5, device="cuda")
+
+        def use(call):
+            s = torch.cuda.Stream()
+            here.stream = s.cuda_stream
+            with torch.cuda.stream(s):
+                for _ in range(40):
+                    call()
+
+        def render():
+            ops._ctx(x)
+            time.sleep(0.001)
+
+        ts = [threading.Thread(target=use, args=(c,)) for c in (lambda: optim.grad_norm([x]),) * 3 + (render,)]
+        [t.start() for t in ts]
+        [t.join() for t in ts]
+        print(len(calls), len(torn), torn[:3])
+    """)
+    assert out.split()[:2] == ["120", "0"], out
+
+
+def test_two_threads_step_as_one_after_the_other():
+    # Clipped steps (two launches each) of two optimizers, norms and clippings in two threads on two streams, against
+    # the same ones one thread after the other.
+    def job(k, seed):
+        torch.manual_seed(seed)
+        out, s = [], torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            gen = torch.Generator(device="cuda").manual_seed(seed)
+            ps = [torch.randn(n, device="cuda", generator=gen) for n in (200_000, 31, 5000)]
+            opt = optim.AdamW(ps, state_bits=8 if k else 32, max_grad_norm=0.5 + k, seed=seed, learning_rate=1e-2)
+            for _ in range(60):
+                gs = [torch.sin(p * 3) * 0.1 for p in ps]
+                out.append(opt.step(gs))
+                out.append(optim.clip_grad_norm_(gs, 0.01))
+                out.append(optim.grad_norm(gs))
+            s.synchronize()
+        return [torch.stack(out)] + ps
+
+    serial = [job(k, 40 + k) for k in range(2)]
+    found, errors = [None, None], []
+
+    def run(k):
+        try:
+            found[k] = job(k, 40 + k)
+        except Exception as e:  # shown below, in the test's own thread
+            errors.append(e)
+
+    old = sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    try:
+        ts = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+        [t.start() for t in ts]
+        [t.join() for t in ts]
+    finally:
+        sys.setswitchinterval(old)
+    assert not errors, errors
+    for a, b in zip(serial, found):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_launch_counts_and_times_hold_the_optimizers_kernels():
+    from diffrast import _lib
+    p = torch.randn(40_000, device="cuda")
+    opt = optim.AdamW([p], max_grad_norm=1.0)
+    n = _lib.launch_count(0)
+    _lib.set_timing(True, 0)
+    opt.step([torch.randn_like(p)])
+    _lib.sync(0)
+    times = _lib.timing_report(0)
+    _lib.set_timing(False, 0)
+    assert _lib.launch_count(0) == n + 2 and times["grad_norm_parts"][0] == 1 and times["adamw"][0] == 1
+
+
+def test_a_failing_call_tells_why():
+    from diffrast import _lib
+    with pytest.raises(_lib.DiffRastError, match="grad_norm: .*unknown type") as e:
+        rows = np.zeros(1, optim._GRAD_ROW)
+        rows["type"] = 9
+        error = optim._rows.norm(optim._context(0), 0, rows.tobytes(), 0.0, torch.zeros(1, device="cuda").data_ptr(), None)
+        _lib.failed(*error, "grad_norm")
+    assert e.value.status == _lib.DR_EINVAL
