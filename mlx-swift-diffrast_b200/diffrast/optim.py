@@ -234,7 +234,8 @@ class AdamW:
     t is counted for each parameter on the device, so a captured step (CUDA
     graph) replays as the next one.  Parameters whose gradient is None are left
     as they are.  Steps of one optimizer must not run at the same time; those
-    of different ones may, from any threads and on any streams.
+    of different ones may, from any threads and on any streams.  A captured step
+    works on this optimizer's buffers: keep it as long as the graph.
     """
 
     def __init__(self, params, learning_rate: Union[float, torch.Tensor] = 1e-3, beta1: float = 0.9,
@@ -316,6 +317,7 @@ class AdamW:
             # A step's own: steps of one optimizer never run side by side.
             self._work = _norm_work(dev.index, count)
         self._ticket_at, self._work_at = self._ticket.data_ptr(), self._work.data_ptr()
+        self._streams = {_rows.stream(dev.index)}
         # What a step's gradients are held against.
         self._shapes = [p.shape for p in self.params]
         self._strides = [p.stride() for p in self.params]
@@ -332,6 +334,15 @@ class AdamW:
         if name.endswith("_scale"):
             return self.state[name][b // BLOCK:b // BLOCK - (-self.params[i].numel() // BLOCK)]
         return self.state[name][b:b + self.params[i].numel()]
+
+    def _use_here(self) -> None:
+        """The buffers, which the caller does not see, are used on the current stream: once this optimizer is gone,
+        their memory waits for that stream as for the one that they were made on."""
+        now = _rows.stream(self._index)
+        if now not in self._streams:
+            self._streams.add(now)
+            for t in (*self.state.values(), self._ticket, self._work):
+                t.record_stream(torch.cuda.current_stream(self._index))
 
     def _step_args(self):
         """(lr, its device tensor or None, max_norm), checked."""
@@ -401,6 +412,7 @@ class AdamW:
             error = _rows.step(None, None, table.tobytes(), *args)
         if error:
             L.failed(*error, "AdamW")
+        self._use_here()
         _written(at)
         return norm
 
@@ -408,6 +420,7 @@ class AdamW:
         """Parameter i's first moment m and root of the second, sqrt(v), as float32 in its shape."""
         p = self.params[i]
         out = []
+        self._use_here()
         for k in ("m", "v") if self.state_bits == 32 else ("m", "r"):
             x = self._flat(k, i).float()
             if self.state_bits == 8:
@@ -436,3 +449,4 @@ class AdamW:
         with torch.cuda.device(self.params[0].device):
             for k, mine in self.state.items():
                 mine.copy_(state[k])
+            self._use_here()

@@ -169,6 +169,14 @@ bool current_stream(long device, void** stream) {
   return false;
 }
 
+// stream(device) -> torch's current stream of the device, as a number.
+PyObject* stream(PyObject*, PyObject* device) {
+  void* now = nullptr;
+  const long index = PyLong_AsLong(device);
+  if (PyErr_Occurred() || !current_stream(index, &now)) return nullptr;
+  return PyLong_FromVoidPtr(now);
+}
+
 // A context serves one call at a time, and keeps the stream and the last error
 // of it.  These contexts are used from here alone, and a call of any thread has
 // its turn from setting the stream to copying the error; it waits for it and
@@ -280,6 +288,7 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows, needs work) or None"},
     {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_last_error, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
+    {"stream", stream, METH_O, "device -> its current stream"},
     {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> None or (status, message)"},
     {"step", (PyCFunction)(void (*)(void))step, METH_FASTCALL, "params, grads, table, ... -> None, (status, message) or False"},
     {nullptr, nullptr, 0, nullptr}};

@@ -141,3 +141,46 @@ def test_a_failing_call_tells_why():
         error = optim._rows.norm(optim._context(0), 0, rows.tobytes(), 0.0, torch.zeros(1, device="cuda").data_ptr(), None)
         _lib.failed(*error, "grad_norm")
     assert e.value.status == _lib.DR_EINVAL
+
+
+# ----------------------------------------------------------------- streams
+
+@pytest.mark.parametrize("use", ["step", "captured", "moments", "load"])
+def test_an_optimizers_memory_waits_for_the_streams_it_was_used_on(use):
+    # Made on one stream and used on another, which is kept busy; then the optimizer goes.  Its buffers' memory must not
+    # be handed out on the first stream while the second is to use them.
+    n = 3_000_001
+    p, g = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+    ref = optim.AdamW([p.clone()], learning_rate=0.1)
+    ref.step([g])
+    opt = optim.AdamW([p], learning_rate=0.1)
+    saved = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state_dict().items()}
+    here = {t.data_ptr() for t in opt.state.values()}
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):  # kernels loaded and memory at hand: neither is to wait for the stream below
+        ref.moments(0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        if use == "captured":
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                opt.step([g])
+            graph.replay()
+        torch.cuda._sleep(300_000_000)
+        if use == "step":
+            opt.step([g])
+        elif use == "moments":
+            out = opt.moments(0)
+        elif use == "load":
+            opt.load_state_dict(saved)
+        elif use == "captured":
+            graph.replay()
+    busy = not s.query()
+    del opt
+    other = [torch.full((n + k,), math.nan, device="cuda") for k in range(-300, 300, 150) for _ in range(2)]
+    assert busy and not here & {t.data_ptr() for t in other}
+    torch.cuda.synchronize()
+    if use == "step":
+        assert torch.equal(p, ref.params[0])
+    if use == "moments":
+        assert all(bool((x == 0).all()) for x in out)
