@@ -257,6 +257,8 @@ class AdamW:
         self.params = _check_list(params, "AdamW")
         count = len(self.params)
         for p in self.params:
+            if p.is_neg():
+                raise ValueError("AdamW: a parameter's memory holds it negated (resolve_neg() copies it)")
             if not _dense(p):
                 raise ValueError("AdamW: parameters must fill their memory (they are updated in place)")
         _check_apart(self.params, "AdamW")
@@ -348,7 +350,7 @@ class AdamW:
         """(lr, its device tensor or None, max_norm), checked."""
         lr, dev, top = self.learning_rate, None, self.max_grad_norm
         if isinstance(lr, torch.Tensor):
-            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda or lr.is_neg():
                 raise ValueError("AdamW: a learning_rate tensor must be one float32 on the parameters' device")
             lr, dev = 0.0, lr
         elif not 0.0 <= float(lr) < 1e30:
@@ -374,6 +376,8 @@ class AdamW:
             p = self._dtypes[i]
             if g.dtype not in _TYPES or not (g.dtype == p or torch.float32 in (p, g.dtype)):
                 raise ValueError(f"AdamW: gradient {i} is {g.dtype}, its parameter {p}")
+            if g.is_neg():
+                g = g.detach().resolve_neg()
             if g.stride() != self._strides[i] and not (g.is_contiguous() and self.params[i].is_contiguous()):
                 g = torch.empty_strided(g.shape, self._strides[i], dtype=g.dtype, device=g.device).copy_(g.detach())
             out.append(g)

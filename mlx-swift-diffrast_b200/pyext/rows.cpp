@@ -52,7 +52,7 @@ constexpr uint8_t kFloat = 2, kBfloat = 4;
 
 const DLPackExchangeAPI* api = nullptr;
 PyTypeObject* tensor_type = nullptr;
-PyObject* grad_name = nullptr;
+PyObject *grad_name = nullptr, *is_neg_name = nullptr;
 
 // What a row needs of a tensor; false where it is not a simple one.
 struct Seen {
@@ -84,6 +84,18 @@ bool look(PyObject* o, Seen& s) {
     }
   }
   return true;
+}
+
+// Whether the memory holds the values negated (the imaginary part of a lazily
+// conjugated tensor, which autograd hands out too).  Such a view steps over the
+// real parts, so that it is contiguous, and gets here, with one element alone.
+bool negated(PyObject* o, const Seen& s) {
+  if (s.n != 1) return false;
+  PyObject* is = PyObject_CallMethodNoArgs(o, is_neg_name);
+  if (!is) PyErr_Clear();
+  const bool plain = is == Py_False;
+  Py_XDECREF(is);
+  return !plain;
 }
 
 char* address(const Seen& s) { return static_cast<char*>(s.t.data) + s.t.byte_offset; }
@@ -266,7 +278,7 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     fine = look(grad, g) && g.t.device.device_id == device && g.t.ndim == p.t.ndim &&
            std::equal(g.t.shape, g.t.shape + g.t.ndim, p.t.shape) &&
-           (g.type == p.type || g.type == DR_F32 || p.type == DR_F32);
+           (g.type == p.type || g.type == DR_F32 || p.type == DR_F32) && !negated(grad, g);
     if (fine) {
       rows[i].grad = address(g);
       rows[i].grad_type = g.type;
@@ -313,5 +325,6 @@ PyMODINIT_FUNC PyInit__rows() {
   }
   tensor_type = reinterpret_cast<PyTypeObject*>(type);
   grad_name = PyUnicode_InternFromString("grad");
-  return grad_name ? PyModule_Create(&module) : nullptr;
+  is_neg_name = PyUnicode_InternFromString("is_neg");
+  return grad_name && is_neg_name ? PyModule_Create(&module) : nullptr;
 }

@@ -184,3 +184,53 @@ def test_an_optimizers_memory_waits_for_the_streams_it_was_used_on(use):
         assert torch.equal(p, ref.params[0])
     if use == "moments":
         assert all(bool((x == 0).all()) for x in out)
+
+
+# ------------------------------------------------- lazily negated gradients
+
+def negated(shape, value):
+    """A tensor whose memory holds -value, as the imaginary part of a conjugated one."""
+    x = torch.full(shape, -value, device="cuda")
+    t = torch.complex(torch.zeros_like(x), x).conj().imag
+    assert t.is_neg() and bool((t == value).all())
+    return t
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1, 1), (3,), (2, 5)])
+def test_a_lazily_negated_gradient_is_taken_at_its_value(bits, shape):
+    g = negated(shape, -2.0)
+    p, q = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+    a, b = (optim.AdamW([x], learning_rate=0.1, state_bits=bits, max_grad_norm=0.5) for x in (p, q))
+    na, nb = a.step([g]), b.step([torch.full(shape, -2.0, device="cuda")])
+    assert torch.equal(p, q) and bool((p > 0).all()) and torch.equal(na, nb)
+    assert torch.equal(a.moments(0)[0], b.moments(0)[0])
+    assert torch.equal(optim.grad_norm([g]), nb)
+
+
+def test_the_gradient_of_one_angle():
+    # Autograd gives a one-element leaf such a gradient as it is.
+    def step(negate):
+        b = torch.ones(1, device="cuda", requires_grad=True)
+        z = torch.complex(torch.ones(1, device="cuda"), b)
+        (z.conj() * torch.tensor([2.0 + 3.0j], device="cuda")).abs().sum().backward()
+        if negate:
+            b.grad = b.grad.resolve_neg()
+        up = float(b.grad) > 0
+        optim.AdamW([b], learning_rate=0.1, weight_decay=0.0).step()
+        return float(b.detach()), up
+    a, up = step(False)
+    assert (a < 1) == up and a == step(True)[0]
+
+
+def test_clipping_a_lazily_negated_gradient_scales_it():
+    g = negated((1,), 3.0)
+    assert float(optim.clip_grad_norm_([g], 1.5)) == 3.0
+    assert abs(float(g) - 1.5) <= 3 * AO.U * 1.5 + 1.5 * 1e-6 / 3
+
+
+def test_lazily_negated_parameters_and_learning_rates_are_refused():
+    with pytest.raises(ValueError, match="negated"):
+        optim.AdamW([negated((1,), 1.0)])
+    with pytest.raises(ValueError, match="learning_rate"):
+        optim.AdamW([torch.zeros(3, device="cuda")], learning_rate=negated((1,), 1.0))
