@@ -532,7 +532,9 @@ DR_API dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int coun
 
 /* dr_grad_norm, then every element times min(1, max_norm / (norm + 1e-6)) in
  * place (nothing is written when that factor is 1).  A NaN or infinite norm
- * gives the factors NaN and 0 that the formula does. */
+ * gives the factors NaN and 0 that the formula does.  The factor is formed from
+ * the norm in 64 bits: finite gradients whose norm is infinite as a float are
+ * scaled all the same. */
 DR_API dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count,
                             double max_norm, float* norm, void* work);
 
@@ -570,7 +572,7 @@ typedef struct dr_adamw_tensor {
  * the step, or `lr` when lr_device is NULL).
  * max_norm > 0: coef = min(1, max_norm / (norm + 1e-6)) with *norm (device, out)
  * the norm over the step's gradients, `work` as for dr_grad_norm; a step whose
- * norm is not finite changes nothing but *norm.  max_norm == 0: coef = 1, norm
+ * *norm is not finite changes nothing else.  max_norm == 0: coef = 1, norm
  * and work may be NULL.
  * state_bits = 8: m is rounded to nearest.  sqrt(v) is rounded to one of its two
  * neighbours, to the upper one with the probability of its distance from the

@@ -487,7 +487,7 @@ __device__ __forceinline__ bool begin_step(const AdamHyper& h, float& coef) {
   const double norm = norm_of<THREADS>(h.part, h.parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *h.norm = (float)norm;
   coef = clip_factor(norm, h.max_norm);
-  return isfinite(norm);  // the same in every block
+  return isfinite((float)norm);  // by the norm that the caller sees; the same in every block
 }
 
 // One more to *count, and what it was.  Released and acquired: the reads that a

@@ -187,8 +187,9 @@ def grad_norm(grads) -> torch.Tensor:
 def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
     """Scales `grads` (the gradients themselves, as grad_norm takes them) in
     place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had.
-    The factor stays on the device.  A NaN or infinite norm gives what the
-    formula does."""
+    The factor stays on the device, formed from the norm in 64 bits.  A NaN or
+    infinite norm gives what the formula does; finite gradients whose norm is
+    beyond float32, and returned as infinite, are scaled all the same."""
     ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     max_norm = float(max_norm)
     if ts and not 0.0 < max_norm < 1e300:
@@ -229,7 +230,7 @@ class AdamW:
       rounded from there; without it, updates below half a step of their type
       are lost.
     max_grad_norm: clip by the norm over all gradients of the step.  A step whose
-      norm is not finite changes nothing.
+      norm, as returned, is not finite changes nothing.
 
     t is counted for each parameter on the device, so a captured step (CUDA
     graph) replays as the next one.  Parameters whose gradient is None are left

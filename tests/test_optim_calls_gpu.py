@@ -18,6 +18,10 @@ from diffrast import optim
 pytestmark = pytest.mark.gpu
 
 
+def f64(t):
+    return t.detach().double().cpu().numpy().reshape(-1)
+
+
 def fresh_python(code):
     """Runs `code` in a process of its own."""
     paths = os.pathsep.join([ROOT, os.path.join(ROOT, "mlx-swift-diffrast_b200"), os.path.join(ROOT, "tests")])
@@ -234,3 +238,37 @@ def test_lazily_negated_parameters_and_learning_rates_are_refused():
         optim.AdamW([negated((1,), 1.0)])
     with pytest.raises(ValueError, match="learning_rate"):
         optim.AdamW([torch.zeros(3, device="cuda")], learning_rate=negated((1,), 1.0))
+
+
+# -------------------------------------------------- norms at float32's border
+
+LARGEST = float(np.finfo(np.float32).max)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [300, 50_000])
+def test_a_step_is_skipped_by_the_norm_that_it_returns(bits, n):
+    # Finite gradients: a norm of 4.2e38 is infinite as a float, one of 3.4028235e38 is the largest float.
+    p = torch.randn(n, device="cuda")
+    old, g = p.clone(), torch.zeros(n, device="cuda")
+    opt = optim.AdamW([p], state_bits=bits, max_grad_norm=1.0)
+    g[:2] = 3e38
+    assert float(opt.step([g])) == math.inf
+    assert torch.equal(p, old) and opt.state["clocks"][0].tolist() == [0, 1, 1, 0]
+    assert all(bool((opt.state[k].float() == 0).all()) for k in opt.state if k != "clocks")
+    g.zero_()
+    g[1] = LARGEST
+    assert float(opt.step([g])) == LARGEST
+    assert opt.state["clocks"][0, 0] == 1 and not torch.equal(p, old) and bool(torch.isfinite(p).all())
+
+
+@pytest.mark.parametrize("n", [3, 50_000])
+def test_clipping_scales_by_the_norm_in_64_bits(n):
+    # The factor, 1 / 5.2e38 for three of 3e38, is 1,373,000 of the smallest float's steps: rounded by 4e-7.
+    x = torch.zeros(n, device="cuda")
+    x[:3] = 3e38
+    value = float(x[0].double())
+    assert float(optim.clip_grad_norm_([x], 1.0)) == math.inf
+    want = value / (value * math.sqrt(3))
+    assert abs(f64(x)[:3] - want).max() <= want * (2.0 ** -150 * value * math.sqrt(3) + 2 * AO.U)
+    assert bool((x[3:] == 0).all())
