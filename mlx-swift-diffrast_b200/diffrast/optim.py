@@ -124,11 +124,11 @@ def _grad_table(ts):
 
 
 def _written(ts) -> None:
-    """Tells autograd that the tensors were changed in place (inference tensors do not count changes)."""
+    """Tells autograd that the tensors (or None) were changed in place; inference tensors do not count changes."""
     try:
         torch.autograd.graph.increment_version(ts)
-    except RuntimeError:
-        torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
+    except (RuntimeError, TypeError):
+        torch.autograd.graph.increment_version([t for t in ts if t is not None and not t.is_inference()])
 
 
 @functools.lru_cache(maxsize=None)
@@ -156,7 +156,10 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
     not contiguous."""
     found = _rows.grads(ts, max_norm > 0.0)
     if found is None:
-        ts = [t if t.is_contiguous() else dense(t) for t in _check_list(ts, what)]
+        ts = _check_list([t for t in ts if t is not None], what)
+        if max_norm > 0.0 and any(t.requires_grad and t.is_leaf for t in ts):
+            raise ValueError(f"{what}: gradients expected, not the parameters (a tensor that requires grad was given)")
+        ts = [t if t.is_contiguous() else dense(t) for t in ts]
         if max_norm > 0.0:
             _check_apart(ts, what)
         found = ts[0].get_device(), _grad_table(ts).tobytes(), True
@@ -178,18 +181,20 @@ def _norm_call(ts, what: str, max_norm: float, dense) -> torch.Tensor:
 def grad_norm(grads) -> torch.Tensor:
     """The 2-norm over all elements of `grads` (a tensor or a sequence of
     tensors, in any mix of float32, bfloat16 and float16): a float32 scalar on
-    their device, the same from run to run.  Squares are summed in 64 bits, so
-    the norm is finite wherever float32 holds it."""
+    their device, the same from run to run.  None, the gradient of a leaf that
+    nothing reached, is passed over.  Squares are summed in 64 bits, so the norm
+    is finite wherever float32 holds it."""
     ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     return _norm_call(ts, "grad_norm", 0.0, lambda t: t if _dense(t) else t.detach().contiguous())
 
 
 def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
-    """Scales `grads` (the gradients themselves, as grad_norm takes them) in
-    place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had.
-    The factor stays on the device, formed from the norm in 64 bits.  A NaN or
-    infinite norm gives what the formula does; finite gradients whose norm is
-    beyond float32, and returned as infinite, are scaled all the same."""
+    """Scales `grads` (the gradients themselves, as grad_norm takes them; unlike
+    torch's function of this name it refuses parameters) in place by
+    min(1, max_norm / (norm + 1e-6)) and returns the norm they had.  The factor
+    stays on the device, formed from the norm in 64 bits.  A NaN or infinite norm
+    gives what the formula does; finite gradients whose norm is beyond float32,
+    and returned as infinite, are scaled all the same."""
     ts = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     max_norm = float(max_norm)
     if ts and not 0.0 < max_norm < 1e300:

@@ -52,7 +52,7 @@ constexpr uint8_t kFloat = 2, kBfloat = 4;
 
 const DLPackExchangeAPI* api = nullptr;
 PyTypeObject* tensor_type = nullptr;
-PyObject *grad_name = nullptr, *is_neg_name = nullptr;
+PyObject *grad_name, *is_neg_name, *requires_grad_name, *is_leaf_name;
 
 // What a row needs of a tensor; false where it is not a simple one.
 struct Seen {
@@ -107,27 +107,41 @@ PyObject** items(PyObject* o, Py_ssize_t& n) {
   return PySequence_Fast_ITEMS(o);
 }
 
-// grads(tensors, apart) -> (device index, dr_grad_tensor rows as bytes, whether
-// the norm needs work), or None.  apart: also None where two tensors share memory.
+// Whether o is a leaf that autograd differentiates for: a parameter, no gradient.
+bool is_parameter(PyObject* o) {
+  PyObject* requires_grad = PyObject_GetAttr(o, requires_grad_name);
+  PyObject* leaf = requires_grad == Py_False ? Py_NewRef(Py_False) : PyObject_GetAttr(o, is_leaf_name);
+  PyErr_Clear();
+  const bool gradient = requires_grad && leaf == Py_False;
+  Py_XDECREF(requires_grad);
+  Py_XDECREF(leaf);
+  return !gradient;
+}
+
+// grads(tensors, written) -> (device index, dr_grad_tensor rows as bytes, whether the norm needs work), or None.
+// None in the list is passed over.  written: also None where two tensors share memory, or one is a parameter.
 PyObject* grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  Py_ssize_t n = 0;
-  PyObject** it = nargs == 2 ? items(args[0], n) : nullptr;
-  if (!it || n == 0) Py_RETURN_NONE;
+  Py_ssize_t items_n = 0, n = 0;
+  PyObject** it = nargs == 2 ? items(args[0], items_n) : nullptr;
+  for (Py_ssize_t i = 0; it && i < items_n; ++i) n += it[i] != Py_None;
+  if (n == 0) Py_RETURN_NONE;
+  const bool written = PyObject_IsTrue(args[1]) == 1;
   PyObject* bytes = PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(dr_grad_tensor));
   if (!bytes) return nullptr;
   auto* rows = reinterpret_cast<dr_grad_tensor*>(PyBytes_AS_STRING(bytes));
   int32_t device = -1;
   int64_t rounded = 0;
   bool fine = true;
-  for (Py_ssize_t i = 0; fine && i < n; ++i) {
+  for (Py_ssize_t i = 0, row = 0; fine && i < items_n && row < n; ++i) {
+    if (it[i] == Py_None) continue;
     Seen s;
-    fine = look(it[i], s) && (i == 0 || s.t.device.device_id == device);
+    fine = look(it[i], s) && (row == 0 || s.t.device.device_id == device) && !(written && is_parameter(it[i]));
     if (!fine) break;
     device = s.t.device.device_id;
-    rows[i] = {address(s), s.n, s.type, 0};
+    rows[row++] = {address(s), s.n, s.type, 0};
     rounded += (s.n + 2047) / 2048 * 2048;
   }
-  if (fine && n > 1 && PyObject_IsTrue(args[1]) == 1) {
+  if (fine && n > 1 && written) {
     struct Span {
       uintptr_t begin, end;
     };
@@ -298,7 +312,7 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyMethodDef methods[] = {
-    {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, apart -> (device, rows, needs work) or None"},
+    {"grads", (PyCFunction)(void (*)(void))grads, METH_FASTCALL, "tensors, written -> (device, rows, needs work) or None"},
     {"bind", bind, METH_VARARGS, "addresses of dr_ctx_set_stream, dr_last_error, dr_grad_norm, dr_clip_grad_norm, dr_adamw_step"},
     {"stream", stream, METH_O, "device -> its current stream"},
     {"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, "ctx, device, rows, max_norm, norm, work -> None or (status, message)"},
@@ -326,5 +340,7 @@ PyMODINIT_FUNC PyInit__rows() {
   tensor_type = reinterpret_cast<PyTypeObject*>(type);
   grad_name = PyUnicode_InternFromString("grad");
   is_neg_name = PyUnicode_InternFromString("is_neg");
-  return grad_name && is_neg_name ? PyModule_Create(&module) : nullptr;
+  requires_grad_name = PyUnicode_InternFromString("requires_grad");
+  is_leaf_name = PyUnicode_InternFromString("is_leaf");
+  return grad_name && is_neg_name && requires_grad_name && is_leaf_name ? PyModule_Create(&module) : nullptr;
 }

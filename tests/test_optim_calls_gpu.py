@@ -272,3 +272,46 @@ def test_clipping_scales_by_the_norm_in_64_bits(n):
     want = value / (value * math.sqrt(3))
     assert abs(f64(x)[:3] - want).max() <= want * (2.0 ** -150 * value * math.sqrt(3) + 2 * AO.U)
     assert bool((x[3:] == 0).all())
+
+
+# ---------------------------------------------- parameters and missing leaves
+
+def test_clipping_refuses_parameters():
+    lin = torch.nn.Linear(17, 5).cuda()
+    lin(torch.randn(3, 17, device="cuda")).sum().backward()
+    ps = list(lin.parameters())
+    old = [(p.detach().clone(), p.grad.clone()) for p in ps]
+    strided = torch.zeros(4, 6, device="cuda").t().requires_grad_()
+    for given in (lin.parameters(), ps, tuple(ps), ps[0], [ps[0].grad, ps[1]], [ps[0].grad, None, strided]):
+        with pytest.raises(ValueError, match="not the parameters"):
+            optim.clip_grad_norm_(given, 1e-3)
+    for p, (w, g) in zip(ps, old):
+        assert torch.equal(p.detach(), w) and torch.equal(p.grad, g)
+    assert float(optim.grad_norm(ps)) > 0  # nothing is written
+
+
+def test_clipping_takes_gradients_that_are_differentiated_again():
+    w = torch.randn(50, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    old, n = f64(g), float(optim.grad_norm([g]).detach())
+    optim.clip_grad_norm_([g], 0.5 * n)
+    assert np.abs(f64(g) - old * (0.5 * n / (n + 1e-6))).max() <= 5 * AO.U * np.abs(old).max()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_missing_gradients_are_passed_over(strided):
+    gs = [torch.randn(300, 7, device="cuda"), torch.randn(9, device="cuda").half()]
+    if strided:
+        gs[0] = torch.randn(7, 300, device="cuda").t()
+    want = optim.grad_norm(gs)
+    for given in ([None, gs[0], None, gs[1]], (gs[0], gs[1], None)):
+        assert torch.equal(optim.grad_norm(given), want)
+    old, version = [g.clone() for g in gs], gs[0]._version
+    assert torch.equal(optim.clip_grad_norm_([gs[0], None, gs[1]], 1.0), want)
+    optim.clip_grad_norm_(old, 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(gs, old)) and gs[0]._version > version
+    for given in ([None], [None, None]):
+        with pytest.raises(ValueError, match="no tensors"):
+            optim.grad_norm(given)
+        with pytest.raises(ValueError, match="no tensors"):
+            optim.clip_grad_norm_(given, 1.0)
