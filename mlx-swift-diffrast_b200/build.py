@@ -5,7 +5,7 @@
 Objects go to mlx-swift-diffrast_b200/_build/, the shared library to
 mlx-swift-diffrast_b200/diffrast/libdiffrast.so (in-tree, next to the Python
 binding that loads it), the host-side Python extension of the optimizer to
-diffrast/_rows.so.  A file is recompiled when it or any header changed.
+diffrast/_rows.<Python's own suffix>.  A file is recompiled when it or any header changed.
 """
 from __future__ import annotations
 
@@ -89,12 +89,20 @@ def build(force: bool = False, jobs: int = 0, verbose_ptxas: bool = False) -> st
 
 
 ROWS_SRC = os.path.join(PKG, "pyext", "rows.cpp")
-ROWS = os.path.join(PKG, "diffrast", "_rows.so")
+# Named for the Python it is built for, which no other one loads.
+ROWS = os.path.join(PKG, "diffrast", "_rows" + sysconfig.get_config_var("EXT_SUFFIX"))
+UNTAGGED_ROWS = os.path.join(PKG, "diffrast", "_rows.so")  # any Python would load it
 
 
-def build_rows(force: bool = False) -> str:
+def build_rows(force: bool = False):
     """The Python extension of the optimizer's host path (pyext/rows.cpp): host
-    compiler only, linked against nothing."""
+    compiler only, linked against nothing.  None without Python's headers: all but
+    AdamW, grad_norm and clip_grad_norm_ goes without it."""
+    if os.path.exists(UNTAGGED_ROWS):
+        os.remove(UNTAGGED_ROWS)
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        sys.stderr.write("Python.h not found: diffrast/_rows is not built (AdamW, grad_norm, clip_grad_norm_)\n")
+        return None
     if not force and os.path.exists(ROWS) and os.path.getmtime(ROWS) >= max(
             os.path.getmtime(ROWS_SRC), os.path.getmtime(__file__), *[os.path.getmtime(h) for h in _headers()]):
         return ROWS

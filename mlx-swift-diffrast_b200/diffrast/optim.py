@@ -19,8 +19,15 @@ from . import _lib as L
 try:
     from . import _rows
 except ImportError as e:
-    raise ImportError("diffrast/_rows.so is missing or of another Python or torch; build it with "
-                      f"`python mlx-swift-diffrast_b200/build.py` ({e})") from e
+    class _Missing:
+        """In place of the extension, which Adam does not need: says why it is missing at its first use."""
+        reason = str(e)
+
+        def __getattr__(self, name):
+            raise ImportError("AdamW, grad_norm and clip_grad_norm_ need diffrast/_rows, which is missing or of another "
+                              f"Python or torch; build it with `python mlx-swift-diffrast_b200/build.py` ({self.reason})")
+
+    _rows = _Missing()
 from .ops import _ctx, _f32, _ptr
 
 

@@ -1,11 +1,18 @@
 """The many-tensor optimizer's sources and host side, without a GPU: what holds whatever a machine's timing shows."""
 import glob
+import importlib.util
 import os
 import re
+import subprocess
+import sys
+import sysconfig
+import textwrap
 
 from conftest import ROOT
 
-CSRC = os.path.join(ROOT, "mlx-swift-diffrast_b200", "csrc")
+PKG = os.path.join(ROOT, "mlx-swift-diffrast_b200")
+
+CSRC = os.path.join(PKG, "csrc")
 
 
 def functions(*names):
@@ -40,3 +47,45 @@ def test_the_clocks_last_block_is_ordered_behind_the_others_reads():
     body = {re.sub(r"\(.*", "", s, flags=re.S).split()[-1]: b for s, b in functions("adamw.cu")}
     assert "draw(h.ticket)" in body["end_step"] and "atomicAdd" not in body["end_step"]
     assert "atom.acq_rel.gpu" in body["draw"] and '"memory"' in body["draw"]
+
+
+def test_adam_goes_without_the_extension():
+    code = textwrap.dedent("""
+        import sys
+        sys.modules["diffrast._rows"] = None  # its import fails
+        import torch
+        from diffrast import optim
+        opt = optim.Adam((3,), device=torch.device("cpu"))
+        assert opt.bias_corrections() is not None
+        sys.path.insert(0, "examples")
+        import fits
+        for call in (lambda: optim.grad_norm([torch.zeros(3)]), lambda: optim.clip_grad_norm_([torch.zeros(3)], 1.0)):
+            try:
+                call()
+            except ImportError as e:
+                assert "build.py" in str(e)
+            else:
+                raise AssertionError("no extension, and no error")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=PKG)
+    assert r.returncode == 0, r.stderr
+
+
+def builder():
+    spec = importlib.util.spec_from_file_location("diffrast_build_test", os.path.join(PKG, "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def test_the_extension_is_named_for_its_python():
+    from diffrast import optim
+    assert os.path.basename(optim._rows.__file__) == "_rows" + sysconfig.get_config_var("EXT_SUFFIX")
+    assert os.path.samefile(builder().ROWS, optim._rows.__file__)
+
+
+def test_a_build_goes_without_pythons_headers(monkeypatch, tmp_path, capsys):
+    b = builder()
+    monkeypatch.setattr(b.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    assert b.build_rows(force=True) is None
+    assert "Python.h" in capsys.readouterr().err
