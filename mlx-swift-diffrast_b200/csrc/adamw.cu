@@ -688,7 +688,8 @@ extern "C" dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* t, int co
   DR_ENTER(ctx);
   DR_REQUIRE(ctx, count >= 0 && (count == 0 || t), "adamw: null list or count < 0");
   DR_REQUIRE(ctx, state_bits == 32 || state_bits == 8, "adamw: state_bits must be 32 or 8");
-  DR_REQUIRE(ctx, ticket, "adamw: ticket is required");
+  DR_REQUIRE(ctx, ticket && (uintptr_t)ticket % 4 == 0, "adamw: a 4-byte aligned ticket is required");
+  DR_REQUIRE(ctx, (uintptr_t)lr_device % 4 == 0 && (uintptr_t)norm % 4 == 0, "adamw: lr_device or norm is misaligned");
   DR_REQUIRE(ctx, lr_device || (lr >= 0.0 && lr < 1e30), "adamw: lr must be finite and not negative");
   DR_REQUIRE(ctx, beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: betas must be in [0, 1)");
   DR_REQUIRE(ctx, eps >= 0x1p-126 && eps < 1e30, "adamw: eps must be at least 2^-126 and finite");

@@ -314,7 +314,7 @@ size_t dr_grad_norm_work_bytes(const dr_ctx* ctx, int count) {
 
 dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, float* norm, void* work) {
   DR_ENTER(ctx);
-  DR_REQUIRE(ctx, norm, "grad_norm: norm is required");
+  DR_REQUIRE(ctx, norm && (uintptr_t)norm % 4 == 0, "grad_norm: a 4-byte aligned norm is required");
   dr_status st = check_list(ctx, grads, count, "grad_norm");
   if (st != DR_OK) return st;
   const bool small = is_small(grads, count);
@@ -327,7 +327,7 @@ dr_status dr_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, floa
 dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int count, double max_norm, float* norm,
                             void* work) {
   DR_ENTER(ctx);
-  DR_REQUIRE(ctx, norm, "clip_grad_norm: norm is required");
+  DR_REQUIRE(ctx, norm && (uintptr_t)norm % 4 == 0, "clip_grad_norm: a 4-byte aligned norm is required");
   DR_REQUIRE(ctx, max_norm > 0.0 && max_norm < 1e300, "clip_grad_norm: max_norm must be positive and finite");
   dr_status st = check_list(ctx, grads, count, "clip_grad_norm");
   if (st != DR_OK) return st;

@@ -315,3 +315,29 @@ def test_missing_gradients_are_passed_over(strided):
             optim.grad_norm(given)
         with pytest.raises(ValueError, match="no tensors"):
             optim.clip_grad_norm_(given, 1.0)
+
+
+# ------------------------------------------------------------ the C entries
+
+def test_c_entries_refuse_misaligned_scalars():
+    from diffrast import _lib
+    L, c = _lib.lib(), _lib.ctx_for(0)
+    x = torch.zeros(4096, device="cuda")
+    p = x.data_ptr()
+    row = np.zeros(1, optim._GRAD_ROW)
+    row["data"], row["n"] = p, 8
+    step = np.zeros(1, optim._ADAMW_ROW)
+    for k, at in (("param", 0), ("grad", 1024), ("m", 2048), ("v", 3072), ("clock", 4096)):
+        step[k] = p + at
+    step["n"] = 8
+    out = p + 8192
+    for off in (1, 2, 3):
+        assert L.dr_grad_norm(c, row.ctypes.data, 1, out + off, None) == _lib.DR_EINVAL
+        assert b"aligned" in L.dr_last_error(c)
+        assert L.dr_clip_grad_norm(c, row.ctypes.data, 1, 1.0, out + off, None) == _lib.DR_EINVAL
+        for lr, norm, ticket in ((None, None, out + off), (out + off, None, out), (None, out + off, out)):
+            assert L.dr_adamw_step(c, step.ctypes.data, 1, 0.1, lr, 0.9, 0.999, 1e-8, 32, 1.0 if norm else 0.0, norm,
+                                   p + 12288, ticket) == _lib.DR_EINVAL
+            assert b"aligned" in L.dr_last_error(c)
+    torch.cuda.synchronize()
+    assert bool((x == 0).all())
