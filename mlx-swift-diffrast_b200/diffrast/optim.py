@@ -337,6 +337,8 @@ class AdamW:
         self._shapes = [p.shape for p in self.params]
         self._strides = [p.stride() for p in self.params]
         self._dtypes = [p.dtype for p in self.params]
+        # The order of a parameter's elements in memory, which its state follows, where it is not that of its indices.
+        self._layouts = [None if p.is_contiguous() else [list(p.shape), list(p.stride())] for p in self.params]
 
     @staticmethod
     def _memory_order(t: torch.Tensor) -> torch.Tensor:
@@ -450,7 +452,7 @@ class AdamW:
         """The state's buffers (not copies) and what they were made for: save it, or load it into an optimizer of
         the same parameters."""
         return {**self.state, "state_bits": self.state_bits, "counts": [p.numel() for p in self.params],
-                "seed": self.seed}
+                "layouts": self._layouts, "seed": self.seed}
 
     def load_state_dict(self, state: dict) -> None:
         """Copies a state_dict() into this optimizer's buffers, which keep their addresses: a captured step goes on
@@ -459,6 +461,10 @@ class AdamW:
             raise ValueError("AdamW: the state is of other parameters or another state_bits")
         if int(state.get("seed", -1)) != self.seed:
             raise ValueError("AdamW: the state is of another seed")
+        if state.get("layouts", self._layouts) != self._layouts:
+            raise ValueError("AdamW: the state is of parameters with another order in memory")
+        if "master" in state and "master" not in self.state:
+            raise ValueError("AdamW: the state has master weights, which this optimizer does not")
         for k, mine in self.state.items():
             x = state.get(k)
             if not isinstance(x, torch.Tensor) or x.shape != mine.shape or x.dtype != mine.dtype:

@@ -341,3 +341,35 @@ def test_c_entries_refuse_misaligned_scalars():
             assert b"aligned" in L.dr_last_error(c)
     torch.cuda.synchronize()
     assert bool((x == 0).all())
+
+
+# ------------------------------------------------------------- saved states
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_of_another_order_in_memory_is_refused(bits, tmp_path):
+    # States lie in the order of their parameter's memory: a channels-last parameter's are another's.
+    def make(last, **kw):
+        x = torch.arange(2.0 * 3 * 4 * 5, device="cuda").view(2, 3, 4, 5)
+        return optim.AdamW([x.to(memory_format=torch.channels_last) if last else x.clone()], state_bits=bits, **kw)
+    g = torch.randn(2, 3, 4, 5, device="cuda")
+    saved = make(True)
+    saved.step([g])
+    torch.save(saved.state_dict(), tmp_path / "x.pt")
+    state = torch.load(tmp_path / "x.pt")
+    same, other = make(True), make(False)
+    same.load_state_dict(state)
+    assert all(torch.equal(a, b) for a, b in zip(same.moments(0), saved.moments(0)))
+    with pytest.raises(ValueError, match="order"):
+        other.load_state_dict(state)
+    assert other.state["clocks"][0, 0] == 0
+    del state["layouts"]  # of a state saved without them
+    same.load_state_dict(state)
+
+
+def test_a_state_with_master_weights_is_refused_where_there_are_none():
+    p = torch.randn(300, device="cuda").bfloat16()
+    with_master, without = optim.AdamW([p.clone()], master_weights=True), optim.AdamW([p.clone()])
+    with pytest.raises(ValueError, match="master"):
+        without.load_state_dict(with_master.state_dict())
+    with pytest.raises(ValueError, match="master"):
+        with_master.load_state_dict(without.state_dict())
