@@ -543,7 +543,10 @@ DR_API dr_status dr_clip_grad_norm(dr_ctx* ctx, const dr_grad_tensor* grads, int
  * the SQUARE ROOT of the second, and m_scale / v_scale the float factor of each
  * block of 256 elements [ceil(n / 256)]: value = code * scale, scale = (largest
  * magnitude in the block) / 448, 0 for a largest magnitude below 2^-100 and NaN
- * for one that is not finite.  All state is 0 before the first step. */
+ * for one that is not finite.  A gradient whose square a float does not hold
+ * (coef |grad| >= 2^64) makes its block of v NaN, and its param with it; the
+ * block's other params follow at the next step.  (With state_bits = 32 its v is
+ * infinite, and the update 0.)  All state is 0 before the first step. */
 typedef struct dr_adamw_tensor {
   void* param;        /* [n] of param_type, updated in place */
   const void* grad;   /* [n] of grad_type */

@@ -237,7 +237,11 @@ class AdamW:
       sqrt(v) in e4m3 with a float32 scale for each 256 elements, 2 bytes an
       element.  m is rounded to nearest, sqrt(v) stochastically, by bits that
       depend on `seed`, the parameter's place, t and the element alone: a step
-      is reproducible.  One value that is not finite makes its block of 256 NaN.
+      is reproducible.  A state value that is not finite makes its block of 256
+      NaN, and with the next step the block's parameters; a gradient of 2^64 or
+      more (1.8e19, after clipping), whose square float32 does not hold, does so
+      too and makes its parameter NaN at once.  (32-bit states keep an infinite
+      v there, and the parameter stays but for its decay.)
     master_weights: bfloat16 and float16 parameters are kept in float32 too and
       rounded from there; without it, updates below half a step of their type
       are lost.

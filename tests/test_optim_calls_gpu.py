@@ -373,3 +373,36 @@ def test_a_state_with_master_weights_is_refused_where_there_are_none():
         without.load_state_dict(with_master.state_dict())
     with pytest.raises(ValueError, match="master"):
         with_master.load_state_dict(without.state_dict())
+
+
+# ----------------------------------------------- gradients beyond 2^64
+
+@pytest.mark.parametrize("size", [1.8e19, 1.9e19, 3e38])
+def test_gradients_whose_squares_float32_does_not_hold(size):
+    # 32-bit states: v is infinite, the update 0.  8-bit states: the block of v is NaN and the element's parameter at
+    # once, the block's others with the next step, other blocks never.
+    p0 = torch.randn(700, device="cuda")
+    g = torch.randn(700, device="cuda")
+    g[5] = size
+    held = size < 2.0 ** 64
+    p = p0.clone()
+    opt = optim.AdamW([p], learning_rate=1e-2)
+    opt.step([g])
+    assert bool(torch.isfinite(p).all()) and bool(torch.isfinite(opt.state["v"][5])) == held
+    if not held:
+        assert abs(float(p[5]) - float(p0[5]) * (1 - 1e-4)) <= 3 * AO.U * abs(float(p0[5]))
+    p = p0.clone()
+    opt = optim.AdamW([p], learning_rate=1e-2, state_bits=8)
+    opt.step([g])
+    m, r = opt.moments(0)
+    assert bool(torch.isfinite(m).all()) and bool(torch.isfinite(r[256:]).all())
+    assert bool(torch.isnan(r[:256]).all()) != held and bool(torch.isfinite(r[:256]).all()) == held
+    assert bool(torch.isnan(p[5])) != held and bool(torch.isfinite(p[:5]).all()) and bool(torch.isfinite(p[6:]).all())
+    opt.step([torch.zeros_like(g)])
+    assert bool(torch.isnan(p[:256]).all()) != held and bool(torch.isfinite(p[256:]).all())
+    # clipped, the same gradient is an ordinary one
+    p = p0.clone()
+    opt = optim.AdamW([p], learning_rate=1e-2, state_bits=8, max_grad_norm=1.0)
+    for _ in range(2):
+        opt.step([g])
+    assert bool(torch.isfinite(p).all()) and bool(torch.isfinite(opt.moments(0)[1]).all())
