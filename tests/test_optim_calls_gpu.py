@@ -406,3 +406,119 @@ def test_gradients_whose_squares_float32_does_not_hold(size):
     for _ in range(2):
         opt.step([g])
     assert bool(torch.isfinite(p).all()) and bool(torch.isfinite(opt.moments(0)[1]).all())
+
+
+# ------------------------------------------ betas, eps, a changing rate, size
+
+U = AO.U
+TINY = 2.0 ** -149
+
+
+def exact(p, g, m, v, t, lr, b1, b2, eps, wd, coef, clipped):
+    """One step in 64 bits from the float32 values p, m and v (with 8-bit states v is r * r, one rounding more): (p, m,
+    r) and how far float32 may be from them, each rounding half a step U.
+    m: beta's, the product's, the sum's; (1 - beta)'s, the product's, the sum's, with clipping the factor's and g's.
+    v: the same, and the square's; clipping counts twice.  p: 1 - lr wd, its product; of the update the factors' two, two
+    products, the sum with eps, the quotient (8 bits: the product with eps's sum is fused, the reciprocal is two, its
+    product is fused), and what m and r carry; the last sum.  Products below float32's normal range lose TINY."""
+    c = 2 if clipped else 0
+    g = g * coef
+    a, b = np.abs(b1 * m), np.abs((1 - b1) * g)
+    x, y = b2 * v, (1 - b2) * g * g
+    m2, v2, r2 = b1 * m + (1 - b1) * g, x + y, np.sqrt(x + y)
+    dm, dv = U * (3 * a + (3 + c) * b) + 2 * TINY, U * (4 * x + (4 + 2 * c) * y) + 3 * TINY
+    dr = np.maximum(np.sqrt(v2 + dv) - r2, r2 - np.sqrt(np.maximum(v2 - dv, 0))) + U * r2
+    root, step = math.sqrt(1 - b2 ** t), lr / (1 - b1 ** t)
+    denom = r2 / root + eps
+    upd = step * m2 / denom
+    p2 = p * (1 - lr * wd) - upd
+    # 1e-5: the products of these errors
+    dp = (2 * U * np.abs(p) + step * dm / denom + np.abs(upd) * (6 * U + dr / (r2 + eps * root))) * (1 + 1e-5)
+    return (p2, m2, r2), (dp + U * np.abs(p2) + TINY, dm, dr)
+
+
+def grads_like(rng, n, dtype):
+    x = rng.normal(size=n) * 10.0 ** rng.uniform(-4, 0, size=n) * (rng.random(n) >= 0.3)
+    return torch.from_numpy(x).to("cuda", dtype)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [None, 0.05])
+@pytest.mark.parametrize("p,g", [(torch.float32, torch.float32), (torch.float16, torch.float16),
+                                 (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("b1,b2,eps", [(0.9, 0.999, 1e-8), (0.0, 0.99, 1e-3), (0.8, 0.0, 1e-2), (0.99, 0.9999, 1.0)])
+def test_adamw_of_any_betas_and_eps(b1, b2, eps, p, g, clip, bits):
+    rng = np.random.default_rng(23)
+    n, wd, lr = 5000, 0.1, 1e-2
+    w = torch.from_numpy(rng.normal(size=n)).to("cuda", p)
+    opt = optim.AdamW([w], learning_rate=lr, beta1=b1, beta2=b2, eps=eps, weight_decay=wd, state_bits=bits,
+                      max_grad_norm=clip, seed=4)
+    for t in range(1, 4):
+        grad = grads_like(rng, n, g)
+        p0, (m0, r0) = f64(w), (f64(x) for x in opt.moments(0))
+        v0 = f64(opt.state["v"][:n]) if bits == 32 else r0 * r0
+        norm = opt.step([grad])
+        coef = AO.clip_factor(float(np.sqrt((f64(grad) ** 2).sum())), clip)
+        assert (norm is None) == (clip is None) and (clip is None or coef < 1)
+        (p2, m2, r2), (dp, dm, dr) = exact(p0, f64(grad), m0, v0, t, lr, b1, b2, eps, wd, coef, clip is not None)
+        half = 0.0 if p == torch.float32 else torch.finfo(p).eps / 2
+        least = 2.0 ** -25 if p == torch.float16 else 0.0
+        assert np.all(np.abs(f64(w) - p2) <= dp + half * (np.abs(p2) + dp) + least)
+        count, b1t, b2t, _ = opt.state["clocks"][0].tolist()
+        assert count == t and abs(b1t - b1 ** t) <= 1e-13 * b1 ** t and abs(b2t - b2 ** t) <= 1e-13 * b2 ** t
+        m1, r1 = (f64(x) for x in opt.moments(0))
+        if bits == 32:
+            assert np.all(np.abs(m1 - m2) <= dm) and np.all(np.abs(r1 - r2) <= dr + U * r2)
+            continue
+        for k, x, dx, got, step in (("m", m2, dm, m1, 2.0 ** -4), ("r", r2, dr, r1, 2.0 ** -3)):
+            scale = f64(opt._flat(k + "_scale", 0))
+            top = np.abs(AO.blocks(x)).max(1)
+            assert np.all(np.abs(scale * 448 - top) <= AO.blocks(dx).max(1) + 2 * U * top)
+            # to nearest: half a step of the grid, 2^-4 of the value or 2^-10; to a neighbour: twice that
+            grid = np.maximum(step * np.abs(x), scale.repeat(256)[:n] * step * 2.0 ** -6)
+            assert np.all(np.abs(got - x) <= grid * (1 + 1e-5) + dx + 4 * U * np.abs(x))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_clipped_step_follows_its_learning_rate(bits):
+    rates = [0.5, 0.03125, 0.0, 0.0078125]
+    p, g = torch.randn(5000, device="cuda"), torch.randn(5000, device="cuda")
+    ref = optim.AdamW([p.clone()], state_bits=bits, max_grad_norm=1.0)
+    lr = torch.tensor(1.0, device="cuda")
+    opt = optim.AdamW([p], learning_rate=lr, state_bits=bits, max_grad_norm=1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step([g])
+    for rate in rates:
+        lr.fill_(rate)
+        graph.replay()
+        ref.learning_rate = rate
+        ref.step([g])
+        assert torch.equal(p, ref.params[0])
+
+
+def test_32_bit_states_and_clipping_beyond_32_bits():
+    # A tensor of 2^32 + 300 elements, 52 GB with gradient and state: its last elements against a small one's.  The squares
+    # of so few bits and their sums are exact in 64 bits: norm and factor do not depend on the order.
+    n = (1 << 32) + 300
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 52 GB")
+    bf16 = torch.bfloat16
+    w, g = torch.zeros(n, device="cuda", dtype=bf16), torch.zeros(n, device="cuda", dtype=bf16)
+    tail, signs = torch.randn(300, device="cuda").to(bf16), torch.randint(-3, 4, (300,), device="cuda").to(bf16)
+    w[-300:], g[-300:], g[:4] = tail, signs, 1.0
+    small_w, small_g = [tail.clone(), torch.zeros(4, device="cuda", dtype=bf16)], [signs.clone(), g[:4].clone()]
+    opt, small = optim.AdamW([w], learning_rate=0.1), optim.AdamW(small_w, learning_rate=0.1)
+    for _ in range(2):
+        assert torch.equal(optim.clip_grad_norm_([g], 2.0), optim.clip_grad_norm_(small_g, 2.0))
+        opt.step([g])
+        small.step(small_g)
+    assert torch.equal(g[-300:], small_g[0]) and torch.equal(g[:4], small_g[1])
+    assert torch.equal(w[-300:], small_w[0]) and torch.equal(w[:4], small_w[1])
+    for k in ("m", "v"):
+        assert torch.equal(opt._flat(k, 0)[-300:], small._flat(k, 0))
+        assert bool((opt._flat(k, 0)[4:1 << 20] == 0).all()) and bool((opt._flat(k, 0)[-4096:-300] == 0).all())
+    assert bool((w[4:1 << 20] == 0).all()) and bool((w[(1 << 32) - 4096:-300] == 0).all())
+    del w, g, opt
+    torch.cuda.empty_cache()
