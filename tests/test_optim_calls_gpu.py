@@ -522,3 +522,68 @@ def test_32_bit_states_and_clipping_beyond_32_bits():
     assert bool((w[4:1 << 20] == 0).all()) and bool((w[(1 << 32) - 4096:-300] == 0).all())
     del w, g, opt
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------ other captures
+
+def test_captured_norms_and_clippings_follow_their_gradients():
+    # 120 tensors (two launches, a work buffer of the graph's), their values changed between replays.
+    gs = [torch.zeros(1 + 37 * i, device="cuda", dtype=(torch.float32, torch.bfloat16)[i % 2]) for i in range(120)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        before = optim.clip_grad_norm_(gs, 1.0)
+        after = optim.grad_norm(gs)
+    for seed in range(3):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        for g in gs:
+            g.copy_(torch.randn(g.shape, device="cuda", generator=gen))
+        same = [g.clone() for g in gs]
+        graph.replay()
+        assert torch.equal(before, optim.clip_grad_norm_(same, 1.0)) and torch.equal(after, optim.grad_norm(same))
+        assert all(torch.equal(a, b) for a, b in zip(gs, same))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_with_strided_and_missing_gradients(bits):
+    def make():
+        torch.manual_seed(5)
+        return [torch.randn(2, 3, 8, 9, device="cuda").to(memory_format=torch.channels_last),
+                torch.randn(40, 30, device="cuda"), torch.randn(7, device="cuda")]
+    gs = [torch.zeros(2, 3, 8, 9, device="cuda"), torch.zeros(30, 40, device="cuda").t(), None]
+    ref = optim.AdamW(make(), state_bits=bits, max_grad_norm=1.0)
+    opt = optim.AdamW(make(), state_bits=bits, max_grad_norm=1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = opt.step(gs)
+    for k in range(3):
+        for g in gs[:2]:
+            g.copy_(torch.randn(g.shape, device="cuda"))
+        graph.replay()
+        assert torch.equal(norm, ref.step(gs))
+    assert all(torch.equal(a, b) for a, b in zip(opt.params, ref.params))
+    assert opt.state["clocks"][:, 0].tolist() == [3, 3, 0]
+
+
+def test_an_optimizer_made_in_inference_mode_steps_outside_it_on_another_stream():
+    with torch.inference_mode():
+        p = torch.ones(300, device="cuda")
+        opt = optim.AdamW([p], learning_rate=0.1, weight_decay=0.0, master_weights=True, max_grad_norm=1.0)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        opt.step([torch.ones(300, device="cuda")])
+        m, _ = opt.moments(0)
+    s.synchronize()
+    assert float((p - 0.9).abs().max()) < 1e-6 and bool((m > 0).all())
+
+
+def test_a_copy_of_an_optimizer_is_refused():
+    import copy
+    p = torch.ones(300, device="cuda")
+    opt = optim.AdamW([p])
+    other = copy.deepcopy(opt)
+    with pytest.raises(ValueError, match="another address"):
+        other.step([torch.ones(300, device="cuda")])
+    assert bool((p == 1).all()) and opt.state["clocks"][0, 0] == 0
