@@ -555,7 +555,7 @@ typedef struct dr_adamw_tensor {
   void* v;
   float* m_scale;
   float* v_scale;
-  double* clock;      /* device [4]: t, beta1^t, beta2^t, unused; 0, 1, 1, 0 before the first step */
+  double* clock;      /* device [4], this tensor's alone: t, beta1^t, beta2^t, unused; 0, 1, 1, 0 before the first step */
   int64_t n;
   double lr_ratio;    /* this tensor's learning rate / the step's */
   double weight_decay;
@@ -571,8 +571,9 @@ typedef struct dr_adamw_tensor {
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr wd) - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * and clock advances to t (state_bits = 8: the quotient is within two units in
- * the last place, and a v below 2^-100 loses bits).  eps is 2^-126 at least.  lr = lr_ratio * (*lr_device, a device float read by
- * the step, or `lr` when lr_device is NULL).
+ * the last place, and a v below 2^-100 loses bits).  eps is 2^-126 at least.
+ * lr = lr_ratio * (*lr_device, a device float read by the step, or `lr` when
+ * lr_device is NULL).
  * max_norm > 0: coef = min(1, max_norm / (norm + 1e-6)) with *norm (device, out)
  * the norm over the step's gradients, `work` as for dr_grad_norm; a step whose
  * *norm is not finite changes nothing else.  max_norm == 0: coef = 1, norm
@@ -585,11 +586,11 @@ typedef struct dr_adamw_tensor {
  * 2^-9 * scale at least.
  * ticket: device uint32, 0 before the first step that uses it, and 0 again
  * after each; steps that may overlap on the GPU need tickets of their own.
- * Tensors must not overlap, nor gradients other tensors' parameters.  Any
- * alignment of the element types is accepted; whole vectors are used where every
- * pointer of a tensor is a multiple of 8 elements.  `tensors` is a host array, read before the call
- * returns; the step reads nothing back and can be captured in a CUDA graph, a
- * replay being the next step. */
+ * Tensors must not overlap, nor gradients the parameters.  Any alignment of the
+ * element types is accepted; whole vectors are used where every pointer of a
+ * tensor is a multiple of 8 elements.  `tensors` is a host array, read before
+ * the call returns; the step reads nothing back and can be captured in a CUDA
+ * graph, a replay being the next step. */
 DR_API dr_status dr_adamw_step(dr_ctx* ctx, const dr_adamw_tensor* tensors, int count, double lr,
                         const float* lr_device, double beta1, double beta2, double eps,
                         int state_bits, double max_norm, float* norm, void* work,

@@ -10,11 +10,12 @@
 // on the device from each tensor's clock (t, b1^t, b2^t), which the step itself
 // advances: nothing in a captured step is fixed to the t of its capture.
 //
-// 32-bit states are bound by memory: 28 bytes an element in fp32, 1150 us for
-// sixteen 2048^2x4 textures (268 M elements, 7.5 GB), 6.5 TB/s.  8-bit states move
-// 16 (fp32) or 10 bytes (16-bit types) and are bound by issue: 355 instructions
-// for a block of 256 elements, most of them the exact roundings, the root, the
-// random bits and the codes; the same textures in fp16 take 475 us, 5.7 TB/s.
+// 32-bit states are bound by memory: 28 bytes an element in fp32, 1150 to 1180 us
+// for sixteen 2048^2x4 textures (268 M elements, 7.5 GB), 6.4 to 6.5 TB/s.  8-bit
+// states move 16 (fp32) or 10 bytes (16-bit types) and are bound by issue: 355
+// instructions for a block of 256 elements, most of them the exact roundings, the
+// root, the random bits and the codes; the same textures in fp16 take 475 us on the
+// device, 5.7 TB/s, and up to 545 in a long run, at the power limit.
 #include <new>
 #include <type_traits>
 
@@ -55,8 +56,9 @@ struct AdamHyper {
   Betas betas;
 };
 
-// The list is a kernel parameter, in two sizes as gradnorm.cu's: a step of two
-// tensors takes 8.2 us with the small block and 11 with the large one.
+// The list is a kernel parameter, in two sizes as gradnorm.cu's: when the second
+// was brought in, a step of two tensors took 8.2 us with the small block and 11
+// with the large one (now 7.9 with the small one, 5.8 on the device).
 template <int CAP>
 struct AdamTable {
   AdamEntry t[CAP];

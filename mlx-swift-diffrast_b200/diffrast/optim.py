@@ -2,7 +2,7 @@
 
 Adam: the step of the example fits (MLXDiffRastExamples/Adam.swift), one
 tensor at a time (dr_adam_step).  AdamW, grad_norm and clip_grad_norm_ (no
-counterpart in the reference): all leaves of a scene in one or two launches,
+counterpart in the reference): all leaves of a scene in a launch or two,
 in fp32, bf16 or fp16, AdamW's states in 32 or in 8 bits.
 """
 from __future__ import annotations
@@ -220,7 +220,7 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
 class AdamW:
     """AdamW over all `params` (a tensor or a sequence of tensors: float32,
     bfloat16, float16, in any mix, on one device) in one launch for each
-    combination of types, updating them in place:
+    combination of types and each 300 tensors of it, updating them in place:
 
         g = min(1, max_grad_norm / (norm + 1e-6)) * grad      (with max_grad_norm)
         m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
@@ -406,7 +406,7 @@ class AdamW:
         """One step from `grads` (one for each parameter, or None to leave it as
         it is; default: the parameters' .grad).  Gradients have their parameter's
         shape and type, or one of the two is float32; they share no memory with
-        other parameters.  Returns the norm of the gradients (a float32 scalar
+        parameters.  Returns the norm of the gradients (a float32 scalar
         on the device) with max_grad_norm, else None."""
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self._index):
