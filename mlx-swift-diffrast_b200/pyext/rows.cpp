@@ -343,13 +343,12 @@ PyMODINIT_FUNC PyInit__rows() {
   PyObject* torch = PyImport_ImportModule("torch");
   PyObject* type = torch ? PyObject_GetAttrString(torch, "Tensor") : nullptr;
   Py_XDECREF(torch);
-  PyObject* capsule = type ? PyObject_GetAttrString(type, "__dlpack_c_exchange_api__") : nullptr;
-  if (!capsule) return nullptr;
-  api = static_cast<const DLPackExchangeAPI*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api"));
-  Py_DECREF(capsule);
-  if (!api) return nullptr;
-  if (api->major != 1 || !api->dltensor_from_py_object_no_sync || !api->current_work_stream) {
-    PyErr_SetString(PyExc_ImportError, "torch's DLPack exchange table is of another version");
+  if (!type) return nullptr;
+  PyObject* capsule = PyObject_GetAttrString(type, "__dlpack_c_exchange_api__");
+  api = capsule ? static_cast<const DLPackExchangeAPI*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api")) : nullptr;
+  Py_XDECREF(capsule);
+  if (!api || api->major != 1 || !api->dltensor_from_py_object_no_sync || !api->current_work_stream) {
+    PyErr_SetString(PyExc_ImportError, "torch has no DLPack exchange table of version 1");
     return nullptr;
   }
   tensor_type = reinterpret_cast<PyTypeObject*>(type);
