@@ -420,6 +420,7 @@ class AdamW:
                 self.eps, self.state_bits, top, None if norm is None else norm.data_ptr(), self._work_at,
                 self._ticket_at)
         at = ps
+        self._use_here()  # before the launches, of which one may fail behind another
         error = _rows.step(ps, grads, self._tab, *args)
         if error is False:
             gs = [p.grad for p in ps] if grads is None else list(grads)
@@ -435,7 +436,6 @@ class AdamW:
             error = _rows.step(None, None, table.tobytes(), *args)
         if error:
             L.failed(*error, "AdamW")
-        self._use_here()
         _written(at)
         return norm
 
@@ -474,6 +474,6 @@ class AdamW:
             if not isinstance(x, torch.Tensor) or x.shape != mine.shape or x.dtype != mine.dtype:
                 raise ValueError(f"AdamW: the state's {k!r} must be {mine.dtype} {tuple(mine.shape)}")
         with torch.cuda.device(self.params[0].device):
+            self._use_here()
             for k, mine in self.state.items():
                 mine.copy_(state[k])
-            self._use_here()
