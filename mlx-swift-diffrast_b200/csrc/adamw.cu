@@ -15,7 +15,7 @@
 // states move 16 (fp32) or 10 bytes (16-bit types) and are bound by issue: 355
 // instructions for a block of 256 elements, most of them the exact roundings, the
 // root, the random bits and the codes; the same textures in fp16 take 475 us on the
-// device, 5.7 TB/s, and up to 545 in a long run, at the power limit.
+// device, 5.7 TB/s, and up to 555 in a long run, at the power limit.
 #include <new>
 #include <type_traits>
 
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kOptThreads) k_adamw(const __grid_constant__ A
 // are on their way while it computes.  One wave of one block of 16 warps to a
 // multiprocessor, two blocks of states to a warp: their instructions interleave
 // and share constants and addresses.  Sixteen textures in fp16: 475 us on the
-// device (545 in a long run, where the power limit holds the clock down); with
+// device (520 to 555 in a long run, where the power limit holds the clock down); with
 // two blocks of 8 warps 500 (565), which start 0.3 us faster on small lists; with
 // one block of states to a warp and three blocks 547; the same with the next
 // elements on their way through shared memory, by asynchronous or bulk copies,

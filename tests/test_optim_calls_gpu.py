@@ -327,7 +327,7 @@ def test_c_entries_refuse_misaligned_scalars():
     row = np.zeros(1, optim._GRAD_ROW)
     row["data"], row["n"] = p, 8
     step = np.zeros(1, optim._ADAMW_ROW)
-    for k, at in (("param", 0), ("grad", 1024), ("m", 2048), ("v", 3072), ("clock", 4096)):
+    for k, at in (("param", 0), ("grad", 512), ("m", 1024), ("v", 1536), ("clock", 2048)):
         step[k] = p + at
     step["n"] = 8
     out = p + 8192
